@@ -15,7 +15,7 @@ LATENT = RANK + ROT             # a cache row: the normalised latent vector, the
 EK, EV = 192, 128               # the expanded form: channels of a key (128 + 64 rotated) and of a value
 SCALE = 1.0 / math.sqrt(EK)     # both forms: scores are those of the expanded keys
 EPS = 1e-6
-MODES = {"neox": 2, "axes": 8, "vision": 24, "interleaved": 40}
+MODES = {"axes": 8, "vision": 24, "interleaved": 40}
 DTYPE = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 BLOCK_BYTES = {"q8_0": 34, "q4_0": 18}      # of 32 values
 
@@ -62,7 +62,7 @@ def draw(rng):
             c = {"op": op, "mode": mode, "type": rng.choice(["f32", "f16"]), "back": rng.random() < 0.5, "n": _log(rng, 1, 4096),
                  "heads": rng.choice([1, 2, 5, 8, 12, 16, 28, 32, 64]), "dim": rng.choice([64, 80, 128]) if mode == "vision" else rng.choice([64, 96, 128, 256])}
         elif op == "append":
-            c = {"op": op, "form": rng.choice(["latent", "axes", "neox"]), "type": rng.choice(["f16", "bf16", "f32"]), "n": _log(rng, 1, 4096), "n_ctx": 8192}
+            c = {"op": op, "form": rng.choice(["latent", "axes", "interleaved"]), "type": rng.choice(["f16", "bf16", "f32"]), "n": _log(rng, 1, 4096), "n_ctx": 8192}
             if c["form"] != "latent":
                 c.update(heads=rng.choice([1, 2, 4, 8, 16]), dim=rng.choice([64, 80, 128]))
         elif op == "latent":
@@ -129,12 +129,11 @@ def _sections(mode, dim):
     return [pairs - 2 * side, side, side, 0]
 
 
-def _freqs(mode, dim, rot, base):
-    """Of every rotated channel pair: which axis' position turns it, and by how much a step (64 bits)."""
-    s = _sections(mode, dim) if mode != "neox" else [rot // 2, 0, 0, 0]
+def _freqs(mode, dim, base):
+    """Of every channel pair: which axis' position turns it, and by how much a step (64 bits)."""
+    s = _sections(mode, dim)
     axis, power = [], []
-    n_pairs = dim // 2 if mode == "vision" else rot // 2
-    for i in range(n_pairs):
+    for i in range(dim // 2):
         k = i % sum(s)
         if mode == "interleaved":
             a = 1 if k % 3 == 1 and k < 3 * s[1] else 2 if k % 3 == 2 and k < 3 * s[2] else 0 if k % 3 == 0 and k < 3 * s[0] else 3
@@ -142,7 +141,7 @@ def _freqs(mode, dim, rot, base):
             a = 0 if k < s[0] else 1 if k < s[0] + s[1] else 2
         axis.append(a)
         power.append(k - sum(s[:a]) if mode == "vision" else i)
-    n_dims = dim // 2 if mode == "vision" else rot
+    n_dims = dim // 2 if mode == "vision" else dim
     return axis, [base ** (-2.0 * p / n_dims) for p in power]
 
 
@@ -188,7 +187,7 @@ def prepare(case, seed):
     if c["op"] == "rope":
         s["x"] = rand(c["n"], c["heads"], c["dim"]).to(DTYPE[c["type"]])
         s["pos"] = _positions(c, g)
-        axis, freq = _freqs(c["mode"], c["dim"], c["dim"], 1e6)
+        axis, freq = _freqs(c["mode"], c["dim"], 1e6)
         s["axis"], s["freq"] = torch.tensor(axis, device="cuda"), torch.tensor(freq, device="cuda", dtype=torch.float64)
     elif c["op"] == "append":
         latent = c["form"] == "latent"
@@ -196,7 +195,7 @@ def prepare(case, seed):
         s["pos"] = _positions(c, g)
         s["index"] = torch.randperm(c["n_ctx"], generator=g, device="cuda")[: c["n"]]     # cells are taken as they come free
         s["cache"] = rand(c["n_ctx"], width).to(DTYPE[c["type"]])
-        axis, freq = _freqs("neox" if latent else c["form"], ROT if latent else c["dim"], ROT if latent else c["dim"], 1e4 if latent else 1e6)
+        axis, freq = _freqs("axes", ROT, 1e4) if latent else _freqs(c["form"], c["dim"], 1e6)
         s["axis"], s["freq"] = torch.tensor(axis, device="cuda"), torch.tensor(freq, device="cuda", dtype=torch.float64)
         if latent:
             s["x"], s["weight"] = rand(c["n"], LATENT), 1 + 0.1 * rand(RANK)
@@ -262,21 +261,18 @@ def _graph(s):
         n, dt = c["n"], DTYPE[c["type"]]
         index = leaf("i64", s["index"], n)
         if c["form"] == "latent":
-            x, pos = leaf("f32", s["x"], LATENT, n), leaf("i32", s["pos"][0], n)
+            x, pos = leaf("f32", s["x"], LATENT, n), leaf("i32", s["pos"], 4 * n)
             weight, cache = leaf("f32", s["weight"], RANK), leaf(c["type"], s["cache"], LATENT, c["n_ctx"])
             row = 4 * LATENT
             low = ctx.mul(ctx.rms_norm(ctx.view_4d(x, RANK, n, 1, 1, row, row * n, row * n, 0), EPS), weight)
-            turned = ctx.rope_ext(ctx.view_4d(x, ROT, 1, n, 1, row, row, row * n, 4 * RANK), pos, None, ROT, MODES["neox"], 32768, 1e4)
+            turned = ctx.rope_multi(ctx.view_4d(x, ROT, 1, n, 1, row, row, row * n, 4 * RANK), pos, None, ROT, _sections("axes", ROT), MODES["axes"], 32768, 1e4)
             rows = ctx.reshape(ctx.concat(ctx.reshape(low, RANK, 1, n), turned, 0), LATENT, n)
             outs = [(ctx.set_rows(cache, rows, index), s["cache"].shape, dt)]
         else:
             h, d = c["heads"], c["dim"]
             k, v = leaf("f32", s["k"], d, h, n), leaf("f32", s["v"], d * h, n)
             kc, vc = leaf(c["type"], s["cache"], d * h, c["n_ctx"]), leaf(c["type"], s["vcache"], d * h, c["n_ctx"])
-            if c["form"] == "neox":
-                turned = ctx.rope_ext(k, leaf("i32", s["pos"][0], n), None, d, MODES["neox"], 32768, 1e6)
-            else:
-                turned = ctx.rope_multi(k, leaf("i32", s["pos"], 4 * n), None, d, _sections(c["form"], d), MODES[c["form"]], 32768, 1e6)
+            turned = ctx.rope_multi(k, leaf("i32", s["pos"], 4 * n), None, d, _sections(c["form"], d), MODES[c["form"]], 32768, 1e6)
             outs = [(ctx.set_rows(kc, ctx.reshape(turned, d * h, n), index), s["cache"].shape, dt), (ctx.set_rows(vc, v, index), s["vcache"].shape, dt)]
     elif c["op"] == "latent":
         h, n, m, q = c["heads"], c["tok"], c["n_kv"], c["seqs"]
@@ -359,7 +355,7 @@ def exact(case, seed):
     s, c = prepare(case, seed), case
 
     def turned(x, pos, dim, mode, base, sign=1):
-        axis, freq = _freqs(mode, dim, dim, base)
+        axis, freq = _freqs(mode, dim, base)
         unit = torch.empty(x.shape[0], dim // 2, dtype=torch.complex128, device="cuda")
         for i, (a, f) in enumerate(zip(axis, freq)):
             turn = sign * f * pos[a].double()
@@ -374,7 +370,7 @@ def exact(case, seed):
         if c["form"] == "latent":
             low = s["x"][:, :RANK].double()
             low = s["weight"].double() * low / (low.pow(2).sum(-1, keepdim=True) / RANK + EPS).sqrt()
-            cache.index_copy_(0, s["index"], torch.cat([low, turned(s["x"][:, None, RANK:], s["pos"], ROT, "neox", 1e4)[:, 0]], -1))
+            cache.index_copy_(0, s["index"], torch.cat([low, turned(s["x"][:, None, RANK:], s["pos"], ROT, "axes", 1e4)[:, 0]], -1))
             return [cache]
         cache.index_copy_(0, s["index"], turned(s["k"], s["pos"], c["dim"], c["form"], 1e6).flatten(1))
         return [cache, s["vcache"].double().index_copy_(0, s["index"], s["v"].double())]
