@@ -37,6 +37,7 @@ extern "C" {
 #define GGML_ROPE_TYPE_NEOX   2
 #define GGML_ROPE_TYPE_MROPE  8
 #define GGML_ROPE_TYPE_VISION 24
+#define GGML_ROPE_TYPE_IMROPE 40
 
 #define QK_K   256
 #define QK4_0  32

@@ -55,6 +55,23 @@ struct ggml_tensor * mxg_rms_norm(mxg_context * ctx, struct ggml_tensor * a, flo
 struct ggml_tensor * mxg_rope_ext(mxg_context * ctx, struct ggml_tensor * a, struct ggml_tensor * pos, struct ggml_tensor * freq_factors,
                                   int n_dims, int mode, int n_ctx_orig, float freq_base, float freq_scale, float ext_factor,
                                   float attn_factor, float beta_fast, float beta_slow);
+/* Rotary positions with several axes (ggml_rope_multi): mode GGML_ROPE_TYPE_MROPE, _IMROPE or
+ * _VISION; pos is i32 [4 * a->ne[2]], the positions of axis 0 (time), then 1, 2 and 3; sections[k]
+ * channel pairs belong to axis k. Angles are taken in 64 bits: pos * freq_base^(-2e/n_dims). NULL
+ * when the arguments do not fit (types, pos length, n_dims, empty sections). */
+struct ggml_tensor * mxg_rope_multi(mxg_context * ctx, struct ggml_tensor * a, struct ggml_tensor * pos, struct ggml_tensor * freq_factors,
+                                    int n_dims, const int sections[4], int mode, int n_ctx_orig, float freq_base, float freq_scale,
+                                    float ext_factor, float attn_factor, float beta_fast, float beta_slow);
+/* Gradient of mxg_rope_ext / mxg_rope_multi for the gradient `a` of their result (ggml_rope_ext_back,
+ * ggml_rope_multi_back): the rotation by the opposite angles, with the same scale. */
+struct ggml_tensor * mxg_rope_ext_back(mxg_context * ctx, struct ggml_tensor * a, struct ggml_tensor * pos, struct ggml_tensor * freq_factors,
+                                       int n_dims, int mode, int n_ctx_orig, float freq_base, float freq_scale, float ext_factor,
+                                       float attn_factor, float beta_fast, float beta_slow);
+struct ggml_tensor * mxg_rope_multi_back(mxg_context * ctx, struct ggml_tensor * a, struct ggml_tensor * pos, struct ggml_tensor * freq_factors,
+                                         int n_dims, const int sections[4], int mode, int n_ctx_orig, float freq_base, float freq_scale,
+                                         float ext_factor, float attn_factor, float beta_fast, float beta_slow);
+/* a and b joined along dim 0..3 (ggml_concat); their other dimensions and types agree, else NULL */
+struct ggml_tensor * mxg_concat(mxg_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b, int dim);
 struct ggml_tensor * mxg_soft_max_ext(mxg_context * ctx, struct ggml_tensor * a, struct ggml_tensor * mask, float scale, float max_bias);
 struct ggml_tensor * mxg_flash_attn_ext(mxg_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k, struct ggml_tensor * v,
                                         struct ggml_tensor * mask, float scale, float max_bias, float logit_softcap);
@@ -74,6 +91,9 @@ void mxg_tensor_get(const struct ggml_tensor * t, void * data, size_t offset, si
 size_t mxg_nbytes(const struct ggml_tensor * t);
 
 enum ggml_status mxg_compute(ggml_backend_t backend, struct ggml_cgraph * g);
+/* as mxg_compute, without waiting (ggml_backend_graph_compute_async): the work is queued on the backend's
+ * stream, in order with earlier graphs; mxg_synchronize waits for it */
+enum ggml_status mxg_compute_async(ggml_backend_t backend, struct ggml_cgraph * g);
 void mxg_synchronize(ggml_backend_t backend);
 void mxg_backend_free(ggml_backend_t backend);
 

@@ -102,6 +102,10 @@ def load():
     _sig(lib, "mxg_glu_split", P, P, P, P, I)
     _sig(lib, "mxg_rms_norm", P, P, P, F)
     _sig(lib, "mxg_rope_ext", P, P, P, P, P, I, I, I, F, F, F, F, F, F)
+    _sig(lib, "mxg_rope_multi", P, P, P, P, P, I, P, I, I, F, F, F, F, F, F)
+    _sig(lib, "mxg_rope_multi_back", P, P, P, P, P, I, P, I, I, F, F, F, F, F, F)
+    _sig(lib, "mxg_rope_ext_back", P, P, P, P, P, I, I, I, F, F, F, F, F, F)
+    _sig(lib, "mxg_concat", P, P, P, P, I)
     _sig(lib, "mxg_soft_max_ext", P, P, P, P, F, F)
     _sig(lib, "mxg_flash_attn_ext", P, P, P, P, P, P, F, F, F)
     _sig(lib, "mxg_argsort", P, P, P, I)
@@ -113,6 +117,7 @@ def load():
     _sig(lib, "mxg_tensor_get", None, P, P, ctypes.c_size_t, ctypes.c_size_t)
     _sig(lib, "mxg_nbytes", ctypes.c_size_t, P)
     _sig(lib, "mxg_compute", I, P, P)
+    _sig(lib, "mxg_compute_async", I, P, P)
     _sig(lib, "mxg_synchronize", None, P)
     _sig(lib, "mxg_backend_free", None, P)
     # llama runner

@@ -212,6 +212,8 @@ void op_glu(OpCtx & c, ggml_tensor * dst);
 void op_rms_norm(OpCtx & c, ggml_tensor * dst, const ggml_tensor * mul /*nullable*/, ggml_tensor * out /*fused dst*/);
 void op_norm(OpCtx & c, ggml_tensor * dst);
 void op_rope(OpCtx & c, ggml_tensor * dst);
+void op_rope_axes(OpCtx & c, ggml_tensor * dst);       // ROPE with several axes, ROPE_BACK (ops_append.hip)
+void op_concat(OpCtx & c, ggml_tensor * dst);
 void op_soft_max(OpCtx & c, ggml_tensor * dst);
 void op_sum_rows(OpCtx & c, ggml_tensor * dst);
 void op_argsort(OpCtx & c, ggml_tensor * dst);
@@ -269,6 +271,15 @@ size_t mmq_act_bytes(const ggml_tensor * mm);                 // f16 activation 
 using UseCount = std::unordered_map<const ggml_tensor *, int>;
 // decode Q/K/V projections + RoPE + KV-cache stores in one launch; returns nodes consumed
 int fuse_qkv_rope_store(OpCtx & c, ggml_cgraph * g, int i, const UseCount & uses);
+// cache rows appended with the rotation on the way, one launch (ops_append.hip): ROPE -> SET_ROWS
+// [, SET_ROWS], or RMS_NORM -> MUL, ROPE -> CONCAT -> SET_ROWS; nodes consumed
+int fuse_append_rows(OpCtx & c, ggml_cgraph * g, int i, const UseCount & uses);
+bool rope_axes_supported(const ggml_tensor * dst);
+bool concat_supported(const ggml_tensor * dst);
+// attention whose keys are wider than its values (ops_fattn_wide.hip)
+bool fa_wide_supported(const ggml_tensor * dst);
+size_t fa_wide_scratch(const ggml_tensor * dst);
+void fa_wide_run(OpCtx & c, ggml_tensor * dst);
 // MoE router chain / expert combine in one launch each (ops_moe.hip); nodes consumed
 int fuse_topk_moe(OpCtx & c, ggml_cgraph * g, int i);
 // the pending q8_0 KV row(s) of KvNewRow: stored by one k_kv_store_q8 launch (ops_qkv.hip)

@@ -10,6 +10,7 @@
 // strides, data pointers, op params) decides replay; capture happens only on the
 // second sighting of a signature so one-shot prefill graphs run eagerly.
 #include "backend.h"
+#include "rope.cuh"
 #include <chrono>
 #include "gemv.h"
 
@@ -535,7 +536,9 @@ static void run_node(OpCtx & c, ggml_tensor * n) {
         case GGML_OP_GLU:        op_glu(c, n); break;
         case GGML_OP_RMS_NORM:   op_rms_norm(c, n, nullptr, n); break;
         case GGML_OP_NORM:       op_norm(c, n); break;
-        case GGML_OP_ROPE:       op_rope(c, n); break;
+        case GGML_OP_ROPE:       if (rope_has_axes(mx_op_param<int32_t>(n, 2))) op_rope_axes(c, n); else op_rope(c, n); break;
+        case GGML_OP_ROPE_BACK:  op_rope_axes(c, n); break;
+        case GGML_OP_CONCAT:     op_concat(c, n); break;
         case GGML_OP_SOFT_MAX:   op_soft_max(c, n); break;
         case GGML_OP_SUM_ROWS:   op_sum_rows(c, n); break;
         case GGML_OP_ARGSORT:    op_argsort(c, n); break;
@@ -752,6 +755,10 @@ static void run_nodes(Stream * s, ggml_cgraph * g) {
             }
         } else if (s->use_fusion) {
             const int i0 = i;
+            if (n->op == GGML_OP_ROPE || n->op == GGML_OP_RMS_NORM) {   // rows appended to a cache, rotated on the way
+                const int k = fuse_append_rows(c, g, i, uses);
+                if (k > 0) { i += k - 1; s->n_fused += k - 1; s->n_nodes_run += k; deferred_retire(s, g, i0, i); continue; }
+            }
             if (n->op == GGML_OP_RMS_NORM && !g_no_moe_fusion) {   // the MoE block's norm + router + top-k (ops_moe.hip)
                 const int k = fuse_moe_router(c, g, i, uses);
                 if (k > 0) { i += k - 1; s->n_fused += k - 1; s->n_nodes_run += k; deferred_retire(s, g, i0, i); continue; }
@@ -848,6 +855,17 @@ void stream_reserve_node(Stream * s, const ggml_tensor * n) {
     stream_reserve(s, scratch_bytes(n), slot, mmq_act_bytes(n));
 }
 
+// A node whose kernel checks nothing further and that supports_op refuses: the graph fails as a
+// whole (GGML_STATUS_FAILED) instead of reading or writing out of range
+static bool node_refused(const ggml_tensor * n) {
+    switch (n->op) {
+        case GGML_OP_CONCAT: case GGML_OP_ROPE_BACK: return !mx_is_empty(n) && !supports_op(n);
+        case GGML_OP_ROPE: return rope_has_axes(mx_op_param<int32_t>(n, 2)) && !mx_is_empty(n) && !supports_op(n);
+        case GGML_OP_FLASH_ATTN_EXT: return n->src[1]->ne[0] != n->src[2]->ne[0] && !mx_is_empty(n) && !supports_op(n);
+        default: return false;
+    }
+}
+
 void graph_compute_impl(Stream * s, ggml_cgraph * g, ggml_status * status) {
     HIP_CHECK(hipSetDevice(s->device));
     staged_writes_wait(s->device, s->stream);
@@ -916,6 +934,11 @@ void graph_compute_impl(Stream * s, ggml_cgraph * g, ggml_status * status) {
 
     size_t need = 0, slot = 0, f16need = 0;
     for (int i = 0; i < g->n_nodes; ++i) {
+        if (node_refused(g->nodes[i])) {   // nothing of the graph has run
+            if (graphs) s->gslots[s->gcur].key.clear();
+            *status = GGML_STATUS_FAILED;
+            return;
+        }
         // (the prefill GEMM -> ADD -> RMS_NORM chain keeps its product in scratch: try_fuse_mm_add)
         const bool add_norm = g->nodes[i]->op == GGML_OP_MUL_MAT && i + 2 < g->n_nodes && g->nodes[i + 1]->op == GGML_OP_ADD &&
                               g->nodes[i + 2]->op == GGML_OP_RMS_NORM && g->nodes[i + 2]->src[0] == g->nodes[i + 1];

@@ -5,6 +5,8 @@
 #include "mx_graph.h"
 #include "common.h"
 
+namespace mx { bool supports_op(const ggml_tensor * op); }   // ops_misc.hip
+
 #include <deque>
 #include <vector>
 #include <unordered_set>
@@ -263,6 +265,61 @@ ggml_tensor * mxg_rope_ext(mxg_context * ctx, ggml_tensor * a, ggml_tensor * pos
     return r;
 }
 
+// the newest tensor of ctx, or nullptr (and the tensor gone) when the backend would refuse it
+static ggml_tensor * accepted(mxg_context * ctx, ggml_tensor * r) {
+    if (mx::supports_op(r)) return r;
+    ctx->tensors.pop_back();
+    return nullptr;
+}
+
+static ggml_tensor * rope_axes_node(mxg_context * ctx, ggml_op op, ggml_tensor * a, ggml_tensor * pos, ggml_tensor * ff, int n_dims,
+                                    const int * sections, int mode, int n_ctx_orig, float freq_base, float freq_scale, float ext_factor,
+                                    float attn_factor, float beta_fast, float beta_slow) {
+    if (!a || !pos || pos->type != GGML_TYPE_I32 || pos->ne[0] != a->ne[2] * (sections ? 4 : 1)) return nullptr;
+    if (sections && !(mode & GGML_ROPE_TYPE_MROPE)) return nullptr;
+    ggml_tensor * r = dup_tensor(ctx, a);
+    int32_t p[15] = {0, n_dims, mode, 0, n_ctx_orig};
+    const float f[6] = {freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow};
+    memcpy(p + 5, f, sizeof(f));
+    if (sections) memcpy(p + 11, sections, 4 * sizeof(int32_t));
+    set_params(r, p, sizeof(p));
+    r->op = op;
+    r->src[0] = a;
+    r->src[1] = pos;
+    r->src[2] = ff;
+    return accepted(ctx, r);
+}
+ggml_tensor * mxg_rope_multi(mxg_context * ctx, ggml_tensor * a, ggml_tensor * pos, ggml_tensor * ff, int n_dims, const int sections[4], int mode,
+                             int n_ctx_orig, float freq_base, float freq_scale, float ext_factor, float attn_factor, float beta_fast, float beta_slow) {
+    if (!sections) return nullptr;
+    return rope_axes_node(ctx, GGML_OP_ROPE, a, pos, ff, n_dims, sections, mode, n_ctx_orig, freq_base, freq_scale, ext_factor, attn_factor,
+                          beta_fast, beta_slow);
+}
+ggml_tensor * mxg_rope_multi_back(mxg_context * ctx, ggml_tensor * a, ggml_tensor * pos, ggml_tensor * ff, int n_dims, const int sections[4], int mode,
+                                  int n_ctx_orig, float freq_base, float freq_scale, float ext_factor, float attn_factor, float beta_fast, float beta_slow) {
+    if (!sections) return nullptr;
+    return rope_axes_node(ctx, GGML_OP_ROPE_BACK, a, pos, ff, n_dims, sections, mode, n_ctx_orig, freq_base, freq_scale, ext_factor, attn_factor,
+                          beta_fast, beta_slow);
+}
+ggml_tensor * mxg_rope_ext_back(mxg_context * ctx, ggml_tensor * a, ggml_tensor * pos, ggml_tensor * ff, int n_dims, int mode, int n_ctx_orig,
+                                float freq_base, float freq_scale, float ext_factor, float attn_factor, float beta_fast, float beta_slow) {
+    return rope_axes_node(ctx, GGML_OP_ROPE_BACK, a, pos, ff, n_dims, nullptr, mode, n_ctx_orig, freq_base, freq_scale, ext_factor, attn_factor,
+                          beta_fast, beta_slow);
+}
+
+ggml_tensor * mxg_concat(mxg_context * ctx, ggml_tensor * a, ggml_tensor * b, int dim) {
+    if (!a || !b || dim < 0 || dim > 3) return nullptr;
+    int64_t ne[4];
+    for (int i = 0; i < 4; ++i) ne[i] = a->ne[i] + (i == dim ? b->ne[i] : 0);
+    ggml_tensor * r = new_impl(ctx, a->type, 4, ne, nullptr, 0);
+    const int32_t p = dim;
+    set_params(r, &p, sizeof(p));
+    r->op = GGML_OP_CONCAT;
+    r->src[0] = a;
+    r->src[1] = b;
+    return accepted(ctx, r);
+}
+
 ggml_tensor * mxg_soft_max_ext(mxg_context * ctx, ggml_tensor * a, ggml_tensor * mask, float scale, float max_bias) {
     ggml_tensor * r = dup_tensor(ctx, a);
     const float p[2] = {scale, max_bias};
@@ -284,7 +341,7 @@ ggml_tensor * mxg_flash_attn_ext(mxg_context * ctx, ggml_tensor * q, ggml_tensor
     r->src[1] = k;
     r->src[2] = v;
     r->src[3] = mask;
-    return r;
+    return k->ne[0] == v->ne[0] ? r : accepted(ctx, r);   // keys wider than the values: the forms of ops_fattn_wide.hip
 }
 
 ggml_tensor * mxg_argsort(mxg_context * ctx, ggml_tensor * a, ggml_sort_order order) {
@@ -398,6 +455,8 @@ ggml_status mxg_compute(ggml_backend_t backend, ggml_cgraph * g) {
     if (backend->iface.synchronize) backend->iface.synchronize(backend);
     return st;
 }
+
+ggml_status mxg_compute_async(ggml_backend_t backend, ggml_cgraph * g) { return backend->iface.graph_compute(backend, g); }
 
 void mxg_synchronize(ggml_backend_t backend) { if (backend->iface.synchronize) backend->iface.synchronize(backend); }
 void mxg_backend_free(ggml_backend_t backend) { backend->iface.free(backend); }

@@ -567,6 +567,7 @@ static bool g_fa_dec1 = getenv("GGML_MI355X_FA_DEC1") != nullptr;   // A/B: the 
 size_t flash_attn_scratch(const ggml_tensor * dst) {
     const ggml_tensor * q = dst->src[0];
     const ggml_tensor * v = dst->src[2];
+    if (dst->src[1]->ne[0] != v->ne[0]) return fa_wide_scratch(dst);
     int64_t nsplit;
     fa_chunk(dst, &nsplit);
     const int64_t rows = q->ne[1] * q->ne[2] * q->ne[3];
@@ -584,12 +585,12 @@ bool flash_attn_supported(const ggml_tensor * dst) {
     const ggml_tensor * v = dst->src[2];
     const ggml_tensor * m = dst->src[3];
     if (q->type != GGML_TYPE_F32 || dst->type != GGML_TYPE_F32) return false;
+    if (k->ne[0] != v->ne[0]) return fa_wide_supported(dst);
     // K and V types: equal, or (round 6) any pair of f16 / q8_0 / q4_0 — the reference's
     // GGML_CUDA_FA_ALL_QUANTS set the fork builds with (fattn.cu:220-260); its own llama-bench
     // line is -ctk q8_0 -ctv f16 (AGENTS.md:166-176)
     auto mixable = [](ggml_type t) { return t == GGML_TYPE_F16 || t == GGML_TYPE_Q8_0 || t == GGML_TYPE_Q4_0; };
     if (k->type != v->type && !(mixable(k->type) && mixable(v->type))) return false;
-    if (k->ne[0] != v->ne[0]) return false;
     const int64_t D = k->ne[0];
     auto plain = [](ggml_type t) { return t == GGML_TYPE_F16 || t == GGML_TYPE_F32; };
     auto coded = [](ggml_type t) { return t == GGML_TYPE_BF16 || t == GGML_TYPE_Q8_0 || t == GGML_TYPE_Q4_0; };
@@ -673,6 +674,7 @@ static bool g_fa_mma_off = getenv("GGML_MI355X_FA_TILE") != nullptr;
 bool fa_dec2_will_run(const ggml_tensor * dst) { return !g_fa_dec1 && g_tune[10] != 1 && fa_dec2_ok(dst); }
 
 void op_flash_attn_ext(OpCtx & c, ggml_tensor * dst) {
+    if (dst->src[1]->ne[0] != dst->src[2]->ne[0]) { kv_new_row_flush(c); fa_wide_run(c, dst); return; }
     if (fa_dec2_will_run(dst)) { fa_dec2_run(c, dst); return; }
     kv_new_row_flush(c);   // (the executor flushes before any other consumer; the other kernels read the cache)
     if (!g_fa_mma_off && !fa_use_dec(dst) && fa_mma_ok(dst)) { fa_mma_run(c, dst); return; }

@@ -8,6 +8,7 @@
 // for reductions.
 #include "backend.h"
 #include "quants.cuh"
+#include "rope.cuh"
 
 #include <cmath>
 
@@ -756,26 +757,6 @@ void op_norm(OpCtx & c, ggml_tensor * dst) {
 // θ_i = p · scale^i accumulated by repeated f32 multiplication, with the host
 // computing scale = powf(base, -2/n_dims) exactly as the CPU does.
 // ---------------------------------------------------------------------------
-struct RopeP {
-    int n_dims, mode;
-    float freq_scale, ext_factor, attn_factor, theta_scale;
-    float corr0, corr1;
-};
-
-__device__ __forceinline__ void rope_cs(float theta_extrap, const RopeP & p, int i0, float * c, float * s) {
-    const float theta_interp = p.freq_scale * theta_extrap;
-    float theta = theta_interp;
-    float mscale = p.attn_factor;
-    if (p.ext_factor != 0.0f) {
-        const float y = (i0 / 2 - p.corr0) / fmaxf(0.001f, p.corr1 - p.corr0);
-        const float ramp_mix = (1.0f - fminf(1.0f, fmaxf(0.0f, y))) * p.ext_factor;
-        theta = theta_interp * (1 - ramp_mix) + theta_extrap * ramp_mix;
-        mscale *= 1.0f + 0.1f * logf(1.0f / p.freq_scale);
-    }
-    *c = cosf(theta) * mscale;
-    *s = sinf(theta) * mscale;
-}
-
 template <typename T, bool NEOX>
 __global__ void k_rope(const char * __restrict__ x, const int32_t * __restrict__ pos, const float * __restrict__ ff,
                        char * __restrict__ y, T4 gx, T4 gy, RopeP p) {
@@ -846,28 +827,11 @@ __global__ __launch_bounds__(256) void k_rope2(const char * __restrict__ x, cons
     }
 }
 
-static float yarn_corr_dim(int n_dims, int n_ctx_orig, float n_rot, float base) {
-    return n_dims * logf(n_ctx_orig / (n_rot * 2 * (float) M_PI)) / (2 * logf(base));
-}
-
 void op_rope(OpCtx & c, ggml_tensor * dst) {
     const ggml_tensor * x = dst->src[0];
     const ggml_tensor * pos = dst->src[1];
     const ggml_tensor * ff = dst->src[2];
-    RopeP p;
-    p.n_dims = mx_op_param<int32_t>(dst, 1);
-    p.mode = mx_op_param<int32_t>(dst, 2);
-    const int n_ctx_orig = mx_op_param<int32_t>(dst, 4);
-    const float freq_base = mx_op_param<float>(dst, 5);
-    p.freq_scale = mx_op_param<float>(dst, 6);
-    p.ext_factor = mx_op_param<float>(dst, 7);
-    p.attn_factor = mx_op_param<float>(dst, 8);
-    const float beta_fast = mx_op_param<float>(dst, 9), beta_slow = mx_op_param<float>(dst, 10);
-    p.theta_scale = powf(freq_base, -2.0f / p.n_dims);
-    const float start = floorf(yarn_corr_dim(p.n_dims, n_ctx_orig, beta_fast, freq_base));
-    const float end = ceilf(yarn_corr_dim(p.n_dims, n_ctx_orig, beta_slow, freq_base));
-    p.corr0 = std::max(0.0f, start);
-    p.corr1 = std::min((float) (p.n_dims - 1), end);
+    const RopeP p = rope_params(dst);
     const int64_t nr = mx_nrows(x);
     const int bs = 64;
     const float * pff = ff ? (const float *) ff->data : nullptr;
@@ -1067,11 +1031,14 @@ bool supports_op(const ggml_tensor * op) {
             return s0->type == GGML_TYPE_F32 && op->type == GGML_TYPE_F32 && s0->nb[0] == 4;
         case GGML_OP_ROPE: {
             const int mode = mx_op_param<int32_t>(op, 2);
+            if (rope_has_axes(mode)) return rope_axes_supported(op);
             if (mode != GGML_ROPE_TYPE_NORMAL && mode != GGML_ROPE_TYPE_NEOX) return false;
             if (!is_f(s0->type) || s0->type != op->type || s0->nb[0] != (size_t) mx_type(s0->type).size) return false;
             if (op->src[2] && op->src[2]->type != GGML_TYPE_F32) return false;
             return s1->type == GGML_TYPE_I32 && s0->ne[0] % 2 == 0;
         }
+        case GGML_OP_ROPE_BACK:      return rope_axes_supported(op);
+        case GGML_OP_CONCAT:         return concat_supported(op);
         case GGML_OP_SOFT_MAX:
             if (s0->type != GGML_TYPE_F32 || op->type != GGML_TYPE_F32 || s0->nb[0] != 4) return false;
             if (s1 && !(s1->type == GGML_TYPE_F32 || s1->type == GGML_TYPE_F16)) return false;

@@ -204,6 +204,31 @@ class Context:
         return self._t(self.lib.mxg_rope_ext(self.ptr, a.ptr, pos.ptr, self._p(ff), n_dims, mode, n_ctx_orig,
                                              freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow))
 
+    def rope_multi(self, a, pos, ff, n_dims, sections, mode, n_ctx_orig, freq_base, freq_scale=1.0, ext_factor=0.0,
+                   attn_factor=1.0, beta_fast=32.0, beta_slow=1.0):
+        """Rotary positions with several axes (ggml_rope_multi): mode 8 (a run of channel pairs an axis), 40 (dealt
+        out in turn) or 24 (vision); pos: i32 [4 * tokens], axis after axis; sections: channel pairs of each axis."""
+        sec = (ctypes.c_int * 4)(*sections)
+        return self._t(self.lib.mxg_rope_multi(self.ptr, a.ptr, pos.ptr, self._p(ff), n_dims, sec, mode, n_ctx_orig,
+                                               freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow))
+
+    def rope_multi_back(self, a, pos, ff, n_dims, sections, mode, n_ctx_orig, freq_base, freq_scale=1.0, ext_factor=0.0,
+                        attn_factor=1.0, beta_fast=32.0, beta_slow=1.0):
+        """The gradient of rope_multi's input, for the gradient `a` of its result."""
+        sec = (ctypes.c_int * 4)(*sections)
+        return self._t(self.lib.mxg_rope_multi_back(self.ptr, a.ptr, pos.ptr, self._p(ff), n_dims, sec, mode, n_ctx_orig,
+                                                    freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow))
+
+    def rope_ext_back(self, a, pos, ff, n_dims, mode, n_ctx_orig, freq_base, freq_scale=1.0, ext_factor=0.0,
+                      attn_factor=1.0, beta_fast=32.0, beta_slow=1.0):
+        """The gradient of rope_ext's input, for the gradient `a` of its result."""
+        return self._t(self.lib.mxg_rope_ext_back(self.ptr, a.ptr, pos.ptr, self._p(ff), n_dims, mode, n_ctx_orig,
+                                                  freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow))
+
+    def concat(self, a, b, dim):
+        """a and b joined along dim (ggml_concat)."""
+        return self._t(self.lib.mxg_concat(self.ptr, a.ptr, b.ptr, dim))
+
     def soft_max_ext(self, a, mask, scale, max_bias=0.0):
         return self._t(self.lib.mxg_soft_max_ext(self.ptr, a.ptr, self._p(mask), scale, max_bias))
 
@@ -225,6 +250,12 @@ class Context:
     def alloc(self, backend):
         if self.lib.mxg_alloc(self.ptr, backend.buft) != 0:
             raise MemoryError("mxg_alloc failed")
+
+    def compute_async(self, backend, graph):
+        """compute() without the wait: queued on the backend's stream, in order with its other graphs."""
+        st = self.lib.mxg_compute_async(backend.ptr, graph)
+        if st != 0:
+            raise RuntimeError(f"graph_compute returned status {st}")
 
     def compute(self, backend, graph):
         st = self.lib.mxg_compute(backend.ptr, graph)
