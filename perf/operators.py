@@ -231,14 +231,17 @@ def _backend():
 
 
 class _Memory:
-    def __init__(self, pointer, shape, kind):
-        self.__cuda_array_interface__ = {"data": (pointer, False), "shape": tuple(shape), "typestr": kind, "version": 2}
+    """A backend tensor's memory for torch; the tensor's context, which owns it, lives as long as a view does."""
+
+    def __init__(self, t, shape, kind):
+        self.owner = t.ctx
+        self.__cuda_array_interface__ = {"data": (t.raw.data, False), "shape": tuple(shape), "typestr": kind, "version": 2}
 
 
 def _torch_view(t, shape, dtype):
     """A backend tensor's memory as a torch tensor."""
     kind = {torch.float32: "<f4", torch.float16: "<f2", torch.bfloat16: "<i2", torch.uint8: "|u1", torch.int32: "<i4", torch.int64: "<i8"}[dtype]
-    v = torch.as_tensor(_Memory(t.raw.data, shape, kind), device="cuda")
+    v = torch.as_tensor(_Memory(t, shape, kind), device="cuda")
     return v.view(torch.bfloat16) if dtype == torch.bfloat16 else v
 
 
