@@ -729,9 +729,9 @@ def test_graph_with_a_refused_node(pkg, ctx, backend):
 
 def test_kernel_choice(pkg, backend):
     """few rows share the keys among the waves; more tokens than a few read the mask once for all heads"""
-    for kw, want in ((dict(heads=16, n=1, m=600), "rows=32 kt=64"), (dict(heads=64, n=1, m=600), "rows=64 kt=64"),
-                     (dict(heads=8, n=40, m=600), "map=1"), (dict(form="expanded", heads=2, n=100, m=600), "rows=128 kt=32"),
-                     (dict(form="expanded", heads=2, n=1, m=600), "rows=32 kt=64")):
+    for kw, want in ((dict(heads=16, n=1, m=600), "rows=32"), (dict(heads=64, n=1, m=600), "rows=64"),
+                     (dict(heads=8, n=40, m=600), "map=1"), (dict(form="expanded", heads=2, n=100, m=600), "rows=128"),
+                     (dict(form="expanded", heads=2, n=1, m=600), "rows=32")):
         c = Case(pkg.Context(), **kw)
         backend.klog(True)
         c.run(backend)
