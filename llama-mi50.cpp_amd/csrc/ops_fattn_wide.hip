@@ -61,20 +61,22 @@ struct FwArgs {
 __device__ __forceinline__ uint4 ldu16(const char * p) { uint4 v; __builtin_memcpy(&v, p, 16); return v; }
 
 // hi + lo = x to 22 bits: the high term truncated, the remainder (exact in f32) truncated again
+__device__ __forceinline__ void split2(float x0, float x1, int j, wh8 & hi, wh8 & lo) {
+    const wh2 h = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    const wh2 l = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(x0 - (float) h[0], x1 - (float) h[1]));
+    hi[j] = h[0]; hi[j + 1] = h[1];
+    lo[j] = l[0]; lo[j + 1] = l[1];
+}
 __device__ __forceinline__ void split8(const float (&x)[8], wh8 & hi, wh8 & lo) {
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        const wh2 h = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(x[j], x[j + 1]));
-        const wh2 l = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(x[j] - (float) h[0], x[j + 1] - (float) h[1]));
-        hi[j] = h[0]; hi[j + 1] = h[1];
-        lo[j] = l[0]; lo[j + 1] = l[1];
-    }
+    for (int j = 0; j < 8; j += 2) split2(x[j], x[j + 1], j, hi, lo);
 }
 
 // A tile in LDS: pieces of 64 channels, each [32 rows][128 B], so that an LDS-DMA instruction of a wave (64 x 16 B,
-// consecutive in LDS) is eight rows of one piece. The eight 16-byte chunks of a row are XORed with swz(row): eight
-// consecutive rows' reads at one chunk, and the transposing reads of four rows x two chunks, fall on different banks
-__device__ __forceinline__ int fw_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+// consecutive in LDS) is eight rows of one piece. The eight 16-byte chunks of a row are XORed with swz(row): two
+// rows cover the 64 banks, so the 16 rows a b128 read takes at one chunk, eight of each parity, get eight places each,
+// and the transposing reads (eight rows x two neighbouring chunks at a time) four pairs for four rows of a parity
+__device__ __forceinline__ int fw_swz(int row) { return (row & 6) | ((row >> 3) & 1); }
 
 __device__ __forceinline__ wh4 lds_tr4(const char * a) {
     return __builtin_bit_cast(wh4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_w4) a));
@@ -82,6 +84,19 @@ __device__ __forceinline__ wh4 lds_tr4(const char * a) {
 
 template <int N> __device__ __forceinline__ void fw_vmcnt() {   // at most N vector memory operations outstanding
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// Workgroup barrier behind this wave's LDS accesses, with LDS-DMA still on its way (__syncthreads waits for that too)
+__device__ __forceinline__ void fw_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// over the four lanes of a row (lane ^ 16, ^ 32, ^ 48), in registers: the swaps exchange rows of 16 (halves of 32) of
+// two copies, so their maximum (sum) is the pair's
+template <bool SUM> __device__ __forceinline__ float fw_row4(float x) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    u2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = SUM ? __uint_as_float(a.x) + __uint_as_float(a.y) : fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return SUM ? __uint_as_float(a.x) + __uint_as_float(a.y) : fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
 }
 
 // element i of a cache row, for the plain loop below
@@ -194,8 +209,7 @@ __device__ __forceinline__ float fw_query(const FwArgs & p, const FwJob & j, int
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
     }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    top = fw_row4<false>(top);
     const int e = top > 0.f && top < INFINITY ? max(-100, min(100, 14 - __builtin_amdgcn_frexp_expf(top))) : 0;
     qp += 128 * s0;
     asm volatile("" : "+v"(qp));
@@ -236,13 +250,12 @@ __device__ __forceinline__ void fw_mask(const FwArgs & p, const FwJob & j, int r
 }
 
 // Online softmax of a lane's row over its 8 keys of the tile and the other three lanes' (the row lies in
-// four): the reference maximum is raised only when a score exceeds it by 5.5 (weights up to 2^8), so O
-// is rescaled on the first tiles only. Scores in s become weights; the row's sum in l is this lane's.
+// four). First the reference maximum: raised only when a score exceeds it by 5.5 (weights up to 2^8), so
+// O is rescaled on the first tiles only. Returns -m log2(e) for the weights e^(s - m).
 template <int ND>
-__device__ __forceinline__ void fw_softmax(wf4 (&s)[2], float & m, float & l, wf4 (&o)[ND], float (&e)[8]) {
+__device__ __forceinline__ float fw_raise(const wf4 (&s)[2], float & m, float & l, wf4 (&o)[ND]) {
     float mt = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    mt = fw_row4<false>(mt);
     const bool raise = mt > m + 5.5f;                           // false while nothing was visible
     if (__any(raise)) {
         const float al = raise ? __builtin_amdgcn_exp2f((m - mt) * FW_L2E) : 1.f;
@@ -251,12 +264,10 @@ __device__ __forceinline__ void fw_softmax(wf4 (&s)[2], float & m, float & l, wf
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= al;
     }
-    const float ms = m == -INFINITY ? 0.f : -m * FW_L2E;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], FW_L2E, ms));
-        l += e[i];
-    }
+    return m == -INFINITY ? 0.f : -m * FW_L2E;
+}
+__device__ __forceinline__ float fw_weight(const wf4 (&s)[2], int i, float ms) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], FW_L2E, ms));
 }
 
 // A row key by key, leaving masked keys out: an infinity or a NaN in V times a weight of 0 is a NaN, and
@@ -310,8 +321,7 @@ __device__ __forceinline__ void fw_again(const FwArgs & p, const FwJob & j, cons
 template <int DK, int DV, int KV, int ND>
 __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, const char * vb, size_t v1, int vd0, int rg0, int d0, float m, float l, wf4 (&o)[ND]) {
     const int lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = fw_row4<true>(l);
     float z = l * 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -368,7 +378,7 @@ template <int KV, int RG> struct FlGeo {
     static constexpr int RING = !QUANT && RG == 2 ? 4 : 3;
     static constexpr int STEPS = QUANT ? 18 * FW_KT * 4 : 0;    // the blocks' steps, [block][key] f32
     static constexpr int BUF = 9 * FW_PIECE + STEPS;
-    static constexpr int DMA = 36 / (2 * RG);                   // LDS-DMA instructions of a wave and tile (RG = 4: 4 or 5)
+    static constexpr int DMA = (36 + 2 * RG - 1) / (2 * RG);    // LDS-DMA instructions of a wave and tile
 };
 
 template <int KV, int RG>
@@ -396,19 +406,12 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
 
     // ---- staging. f16: instruction x of a tile fills rows 8 (x & 3) .. + 7 of piece x >> 2; lane l brings
     // the chunk that belongs at its place, (l % 8) ^ swz(row) of row l / 8
-    const int srow = lane >> 3, ssrc = 16 * ((lane & 7) ^ fw_swz(srow));
-    auto dma = [&](int tile, char * buf) {
-        if constexpr (!QUANT) {
-#pragma unroll
-            for (int i = 0; i < (36 + NW - 1) / NW; ++i) {
-                // a wave keeps to one row group (wave & 3), so one row pointer; eight waves: pieces by halves
-                const int piece = NW == 8 ? 2 * i + (wave >> 2) : i;
-                if (NW == 8 && piece > 8) break;
-                const int row = 8 * (wave & 3) + srow;
-                const char * kr = j.kb + (size_t) min((tile & 0x3FFFFFFF) * FW_KT + row, p.n_kv - 1) * p.k1 + ssrc;
-                __builtin_amdgcn_global_load_lds(kr + 128 * piece, (lds_dma) (buf + piece * FW_PIECE + 1024 * (wave & 3)), 16, 0, 0);
-            }
-        }
+    const int srow = 8 * (wave & 3) + (lane >> 3), ssrc = 16 * ((lane & 7) ^ fw_swz(srow));
+    auto dma_row = [&](int tile) { return j.kb + (size_t) min((tile & 0x3FFFFFFF) * FW_KT + srow, p.n_kv - 1) * p.k1 + ssrc; };
+    // instruction i of a wave: it keeps to one row group (wave & 3); of eight waves, two share one and halve its pieces
+    auto dma = [&](const char * kr, char * buf, int i) __attribute__((always_inline)) {
+        const int piece = NW == 8 ? min(2 * i + (wave >> 2), 8) : i;        // (piece 8 is brought twice)
+        __builtin_amdgcn_global_load_lds(kr + 128 * piece, (lds_dma) (buf + piece * FW_PIECE + 1024 * (wave & 3)), 16, 0, 0);
     };
     // quantised: TPR threads a row take blocks tid % TPR + TPR i through registers
     constexpr int TPR = geo::NT / 32, QI = (18 + TPR - 1) / TPR, QB = qsize_of<QUANT ? KV : GGML_TYPE_Q8_0>();
@@ -426,19 +429,15 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
             }
         }
     };
-    auto store = [&](char * buf, int slot) {
+    auto store = [&](char * buf, int i) __attribute__((always_inline)) {      // the thread's block i
         if constexpr (QUANT) {
             // integers to f16 exactly: 1024 + n has n in its low bits, two at a time
             const int row = tid / TPR, sw = fw_swz(row);
             float * steps = (float *) (buf + 9 * FW_PIECE);
-            float top = 0.f;
-#pragma unroll
-            for (int i = 0; i < QI; ++i) {
+            {
                 const int b = tid % TPR + TPR * i;
                 if (b < 18) {
-                    const float d = h2f(qd[i]);
-                    steps[b * FW_KT + row] = d;
-                    top = fmaxf(top, fabsf(d));
+                    steps[b * FW_KT + row] = h2f(qd[i]);
                     uint32_t w[16];                             // 32 values in order, as f16 pairs
                     if constexpr (KV == GGML_TYPE_Q8_0) {
                         const uint32_t src[8] = {qa[i].x, qa[i].y, qa[i].z, qa[i].w, qb[i].x, qb[i].y, qb[i].z, qb[i].w};
@@ -469,6 +468,13 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
                         *(uint4 *) (kd + 16 * ((4 * (b & 1) + c) ^ sw)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
                 }
             }
+        }
+    };
+    auto store_top = [&](int slot) __attribute__((always_inline)) {
+        if constexpr (QUANT) {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < QI; ++i) top = fmaxf(top, fabsf(h2f(qd[i])));   // (blocks past the row's repeat its last)
             top = wave_max<64>(top);
             if (lane == 0) dtop[slot][wave] = top;
         }
@@ -479,15 +485,23 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
     char * const ring[4] = {t0, t1, t2, t3};
     int id[RING], held = -1;
 #pragma unroll
-    for (int c = 0; c < RING; ++c) {
-        id[c] = c < RING - 1 && (c == 0 || id[c - 1] >= 0) ? tiles.next<ROWS>(p, j) : -1;
+    for (int c = 0; c < RING - 1; ++c) {
+        id[c] = c == 0 || id[c - 1] >= 0 ? tiles.next<ROWS>(p, j) : -1;
         if (id[c] < 0) continue;
-        if constexpr (QUANT) { load(id[c]); store(ring[c], c); }
-        else dma(id[c], ring[c]);
+        if constexpr (QUANT) {
+            load(id[c]);
+#pragma unroll
+            for (int i = 0; i < QI; ++i) store(ring[c], i);
+            store_top(c);
+        } else {
+            const char * kr = dma_row(id[c]);
+#pragma unroll
+            for (int i = 0; i < geo::DMA; ++i) dma(kr, ring[c], i);
+        }
     }
+    id[RING - 1] = id[RING - 2] >= 0 ? tiles.next<ROWS>(p, j) : -1;         // fetched by the first body
     if constexpr (QUANT) {
-        if (id[1] >= 0) held = tiles.next<ROWS>(p, j);
-        if (held >= 0) load(held);
+        if (id[RING - 1] >= 0) { load(id[RING - 1]); held = tiles.next<ROWS>(p, j); }
     }
     wh8 qh[NS], ql[NS];
     const float qsc = fw_query<576, NS>(p, j, r, NS * dh, qh, ql);
@@ -508,64 +522,83 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
 #pragma unroll
     for (int i = 0; i < 4; ++i) va[i] = (4 * dh + p.vpiece) * FW_PIECE + 128 * vrow + 16 * ((2 * i + (ip >> 1)) ^ vsw) + 8 * (ip & 1);
 
-    // ---- the tile in slot C; another takes the place of the one before it
     int par = 0;
-    auto body = [&](auto slot_) {
-        constexpr int C = decltype(slot_)::value, F = (C + RING - 1) % RING, N = (C + RING - 2) % RING;   // free, newest
-        char * const buf = ring[C];
-        // ---- this half's part of S^T
-        wf4 s[2] = {wf4{0.f, 0.f, 0.f, 0.f}, wf4{0.f, 0.f, 0.f, 0.f}};
-        wh8 a[3][2];
-        auto lda = [&](int i) {
+    wf4 s[2], t[2];                                             // the scores of the tile in hand, this half's of the next
+    float ms = 0.f, qf = 1.f;
+    wh8 ph, pl;
+    float e[8];
+    // fragments from LDS are read AK (AV) steps ahead: with eight waves at it a read takes some 250 cycles, a step's
+    // matrix instructions 64. The first ones before the barrier's other business, and before the end of the scores
+    constexpr int AK = QUANT && RG == 4 ? 2 : 4, AV = QUANT && RG == 4 ? 2 : 3;
+    wh8 a[AK + 1][2], v[AV + 1][2];
+    auto lda = [&](const char * buf, int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) a[i % 3][u] = *(const wh8 *) (buf + (i & 1 ? ka1 : ka0) + (i >> 1) * FW_PIECE + 2048 * u);
-        };
-        lda(0);
-        lda(1);
+        for (int u = 0; u < 2; ++u) a[i % (AK + 1)][u] = *(const wh8 *) (buf + (i & 1 ? ka1 : ka0) + (i >> 1) * FW_PIECE + 2048 * u);
+    };
+    auto ldv = [&](const char * buf, int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const char * a_ = buf + va[2 * (b & 1) + c] + (b >> 1) * FW_PIECE;
+            const wh4 v0 = lds_tr4(a_), v1 = lds_tr4(a_ + 2048);
+            v[b % (AV + 1)][c] = wh8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        }
+    };
+    auto ahead = [&](const char * buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < AK; ++i) lda(buf, i);
+    };
+    // this half's part of the scores of the tile in `buf` to the exchange; meanwhile (W) the weights of the tile in
+    // hand, whose values lie in `vbuf`
+    // and a further tile goes to `fbuf`: instruction by instruction here, where the matrix unit hides them (all at once
+    // behind the barrier they took 800 cycles). They run on past the last tile, into places no longer read
+    auto scores = [&](const char * buf, const char * vbuf, char * fbuf, const char * fsrc, auto with) __attribute__((always_inline)) {
+        constexpr bool W = decltype(with)::value;
+        t[0] = t[1] = wf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            if (i + 2 < NS) lda(i + 2);
+            if constexpr (W && !QUANT) { if (i < geo::DMA) dma(fsrc, fbuf, i); }
+            if constexpr (W && QUANT) { if (i % 3 == 0 && i / 3 < QI) store(fbuf, i / 3); }
+            if (i + AK < NS) lda(buf, i + AK);
+            if (W && i >= NS - AV) ldv(vbuf, i - (NS - AV));
             if constexpr (!QUANT) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % 3][u], qh[i], s[u], 0, 0, 0);
+                for (int u = 0; u < 2; ++u) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], t[u], 0, 0, 0);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % 3][u], ql[i], s[u], 0, 0, 0);
+                for (int u = 0; u < 2; ++u) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], t[u], 0, 0, 0);
             } else {
                 // one 32-block a step: its products are whole, then take the block's step
-                wf4 t[2];
+                wf4 x[2];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % 3][u], qh[i], wf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                for (int u = 0; u < 2; ++u) x[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], wf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % 3][u], ql[i], t[u], 0, 0, 0);
+                for (int u = 0; u < 2; ++u) x[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], x[u], 0, 0, 0);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const wf4 d = *(const wf4 *) (buf + 9 * FW_PIECE + 4 * ((NS * dh + i) * FW_KT + 16 * u + 4 * g4));
-                    s[u] += d * t[u];
+                    t[u] += d * x[u];
+                }
+            }
+            if constexpr (W) {
+                if (i < 8) {
+                    e[i] = fw_weight(s, i, ms);
+                    l += e[i];
+                    if constexpr (QUANT) e[i] *= qf;
+                    else if (i & 1) split2(e[i - 1], e[i], i - 1, ph, pl);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        // ---- the halves change places; behind the barrier the ring's oldest tile is free and the next one whole
-        exch[par][wave][0][lane] = s[0];
-        exch[par][wave][1][lane] = s[1];
-        if constexpr (!QUANT) {
-            if (RING == 4 && id[N] >= 0) fw_vmcnt<geo::DMA>();  // all but the newest tile's have landed
-            else fw_vmcnt<0>();
-        }
-        __syncthreads();
-        if constexpr (QUANT) {
-            id[F] = held;
-            if (held >= 0) {
-                store(ring[F], F);
-                held = tiles.next<ROWS>(p, j);
-                if (held >= 0) load(held);
-            }
-        } else {
-            id[F] = id[N] >= 0 ? tiles.next<ROWS>(p, j) : -1;
-            if (id[F] >= 0) dma(id[F], ring[F]);
-        }
-        s[0] += exch[par][wave ^ 1][0][lane];
-        s[1] += exch[par][wave ^ 1][1][lane];
+        exch[par][wave][0][lane] = t[0];
+        exch[par][wave][1][lane] = t[1];
+    };
+    // behind the barrier: the scores of tile `tile` (slot C) whole, the reference maximum; the first fragments of the
+    // tile in `buf` meanwhile
+    auto whole = [&](int tile, const int C, const char * buf) __attribute__((always_inline)) {
+        const wf4 x0 = exch[par][wave ^ 1][0][lane], x1 = exch[par][wave ^ 1][1][lane];
+        __builtin_amdgcn_sched_barrier(0);
+        ahead(buf);
+        s[0] = t[0] + x0;
+        s[1] = t[1] + x1;
         par ^= 1;
         s[0] *= qsc;
         s[1] *= qsc;
@@ -573,72 +606,100 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = p.softcap * tanhf(s[i >> 2][i & 3]);
         }
-        if (id[C] >> 30) fw_mask(p, j, r, id[C] & 0x3FFFFFFF, s);
-        float qf = 1.f;
+        if (tile >> 30) fw_mask(p, j, r, tile & 0x3FFFFFFF, s);
         if constexpr (QUANT) {
             float top = 0.f;
 #pragma unroll
             for (int i = 0; i < NW; ++i) top = fmaxf(top, dtop[C][i]);
-            const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : -1000;
-            if (e > qe) {                                       // the same in every wave; on the first tiles only
-                const float f = __builtin_amdgcn_ldexpf(1.f, max(qe - e, -200));
+            const int x = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : -1000;
+            if (x > qe) {                                       // the same in every wave; on the first tiles only
+                const float f = __builtin_amdgcn_ldexpf(1.f, max(qe - x, -200));
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] *= f;
-                qe = e;
+                qe = x;
             }
             qf = qe == -1000 ? 1.f : __builtin_amdgcn_ldexpf(1.f, 7 - qe);
         }
-        float e[8];
-        fw_softmax<ND>(s, m, l, o, e);
-        wh8 ph, pl;
-        if constexpr (!QUANT) split8(e, ph, pl);
-        else {
+        ms = fw_raise<ND>(s, m, l, o);
+    };
+    // O^T += V^T P^T: keys 4 g4 + 0..3 of the two 16-key blocks a lane, as the scores lie; 32 channels at a
+    // time, so that a term's product does not wait for the other's
+    auto values = [&](const char * buf) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] *= qf;
-        }
-        // ---- O^T += V^T P^T: keys 4 g4 + 0..3 of the two 16-key blocks a lane, as the scores lie
-        wh4 v[3][2];
-        auto ldv = [&](int d) {
-            const char * a_ = buf + va[d & 3] + (d >> 2) * FW_PIECE;
-            v[d % 3][0] = lds_tr4(a_);
-            v[d % 3][1] = lds_tr4(a_ + 2048);
-        };
-        ldv(0);
-        ldv(1);
+        for (int b = 0; b < ND / 2; ++b) {
+            if (b + AV < ND / 2) ldv(buf, b + AV);
+            if constexpr (QUANT) {                              // a 32-block of V: its steps enter the weights
+                const float * sp = (const float *) (buf + 9 * FW_PIECE) + (8 * dh + 2 * p.vpiece + b) * FW_KT + 4 * g4;
+                const wf4 d0 = *(const wf4 *) sp, d1 = *(const wf4 *) (sp + 16);
+                float x[8];
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            if (d + 2 < ND) ldv(d + 2);
-            if constexpr (QUANT) {
-                if (d % 2 == 0) {                               // a 32-block of V: its steps enter the weights
-                    const float * sp = (const float *) (buf + 9 * FW_PIECE) + (8 * dh + 2 * p.vpiece + d / 2) * FW_KT + 4 * g4;
-                    const wf4 d0 = *(const wf4 *) sp, d1 = *(const wf4 *) (sp + 16);
-                    float x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = e[i] * (i < 4 ? d0[i & 3] : d1[i & 3]);
-                    split8(x, ph, pl);
-                }
+                for (int i = 0; i < 8; ++i) x[i] = e[i] * (i < 4 ? d0[i & 3] : d1[i & 3]);
+                split8(x, ph, pl);
             }
-            const wh4 v0 = v[d % 3][0], v1 = v[d % 3][1];
-            const wh8 vf = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[d], 0, 0, 0);
+            o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], ph, o[2 * b], 0, 0, 0);
+            o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], ph, o[2 * b + 1], 0, 0, 0);
+            o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], pl, o[2 * b], 0, 0, 0);
+            o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], pl, o[2 * b + 1], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    // the tile in slot C, its scores in hand, with the next tile's scores on the way: the weights are taken among the
+    // matrix instructions of the next tile's scores, the exchange passes under this tile's values. The barrier then
+    // frees slot C (and tells that the tile after the next is whole)
+    auto body = [&](auto slot_) __attribute__((always_inline)) {
+        constexpr int C = decltype(slot_)::value, C1 = (C + 1) % RING, F = (C + RING - 1) % RING;
+        const char * fsrc = nullptr;
+        if constexpr (!QUANT) fsrc = dma_row(id[F] >= 0 ? id[F] : id[C]);
+        scores(ring[C1], ring[C], ring[F], fsrc, std::true_type{});
+        if constexpr (QUANT) {
+            store_top(F);
+            load(held >= 0 ? held : id[C]);
+        }
+        values(ring[C]);
+        if constexpr (!QUANT) fw_vmcnt<(RING - 3) * geo::DMA>();    // the tile after the next has landed
+        fw_barrier();
+        if constexpr (QUANT) {
+            id[C] = held;
+            held = held >= 0 ? tiles.next<ROWS>(p, j) : -1;
+        } else id[C] = id[F] >= 0 ? tiles.next<ROWS>(p, j) : -1;
+        whole(id[C1], C1, ring[(C + 2) % RING]);                // (fragments read for nothing where no such tile is left)
     };
 
     if constexpr (!QUANT) fw_vmcnt<0>();
     __syncthreads();
-    for (;;) {
-        if (id[0] < 0) break;
-        body(std::integral_constant<int, 0>{});
-        if (id[1] < 0) break;
-        body(std::integral_constant<int, 1>{});
-        if (id[2] < 0) break;
-        body(std::integral_constant<int, 2>{});
-        if constexpr (RING == 4) {
-            if (id[3] < 0) break;
-            body(std::integral_constant<int, 3>{});
+    if (id[0] >= 0) {
+        ahead(t0);
+        scores(t0, t0, nullptr, nullptr, std::false_type{});
+        fw_barrier();
+        whole(id[0], 0, t1);
+        const char * last;
+        for (;;) {
+            last = t0;
+            if (id[1] < 0) break;
+            body(std::integral_constant<int, 0>{});
+            last = t1;
+            if (id[2] < 0) break;
+            body(std::integral_constant<int, 1>{});
+            last = t2;
+            if (id[3 % RING] < 0) break;
+            body(std::integral_constant<int, 2>{});
+            if constexpr (RING == 4) {
+                last = t3;
+                if (id[0] < 0) break;
+                body(std::integral_constant<int, 3>{});
+            }
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            e[i] = fw_weight(s, i, ms);
+            l += e[i];
+            if constexpr (QUANT) e[i] *= qf;
+            else if (i & 1) split2(e[i - 1], e[i], i - 1, ph, pl);
+        }
+        if constexpr (!QUANT) fw_vmcnt<0>();                    // no DMA outlives the workgroup's LDS
+#pragma unroll
+        for (int b = 0; b < AV; ++b) ldv(last, b);
+        values(last);
     }
     if constexpr (QUANT) {
         const float f = qe == -1000 ? 1.f : __builtin_amdgcn_ldexpf(1.f, qe - 7);
@@ -652,7 +713,7 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
 // W waves of NT row groups of 16 each: a K or V fragment from LDS serves NT groups (and both terms), so
 // with NT = 2 the LDS moves half of what the matrix instructions could take.
 template <int NT, int W>
-__global__ __launch_bounds__(64 * W, 2) void k_fattn_expanded(FwArgs p) {
+__global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     constexpr int NS = 6, ND = 8, ROWS = 16 * NT * W, BUF = 5 * FW_PIECE, DMA = 20 / W;
     __shared__ __align__(128) char t0[BUF];
     __shared__ __align__(128) char t1[BUF];
@@ -666,7 +727,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_fattn_expanded(FwArgs p) {
     FwTiles tiles;
     tiles.w0 = 0;
     tiles.window<ROWS>(p, j);
-    const int srow = lane >> 3, ssrc = 16 * ((lane & 7) ^ fw_swz(srow));
+    const int srow = lane >> 3, ssrc = 16 * ((lane & 7) ^ fw_swz(8 * wave + srow));   // (W is even: the same for rb below)
     auto dma = [&](int tile, char * buf) {
 #pragma unroll
         for (int b = 0; b < 4 / W; ++b) {
@@ -702,11 +763,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_fattn_expanded(FwArgs p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) va[i] = 3 * FW_PIECE + 128 * vrow + 16 * ((2 * i + (ip >> 1)) ^ vsw) + 8 * (ip & 1);
 
-    auto body = [&](auto slot_) {
+    auto body = [&](auto slot_) __attribute__((always_inline)) {
         constexpr int C = decltype(slot_)::value, F = (C + 2) % 3, N = (C + 1) % 3;
         char * const buf = ring[C];
         if (id[N] >= 0) fw_vmcnt<DMA>(); else fw_vmcnt<0>();    // this wave's part of the tile
-        __syncthreads();                                        // the tile is whole; the one before it is free
+        fw_barrier();                                           // the tile is whole; the one before it is free
         id[F] = id[N] >= 0 ? tiles.next<ROWS>(p, j) : -1;
         if (id[F] >= 0) dma(id[F], ring[F]);
         wf4 s[NT][2];
@@ -756,8 +817,13 @@ __global__ __launch_bounds__(64 * W, 2) void k_fattn_expanded(FwArgs p) {
         ldv(1);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            const float ms = fw_raise<ND>(s[nt], m[nt], l[nt], o[nt]);
             float e[8];
-            fw_softmax<ND>(s[nt], m[nt], l[nt], o[nt], e);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = fw_weight(s[nt], i, ms);
+                l[nt] += e[i];
+            }
             split8(e, ph[nt], pl[nt]);
         }
 #pragma unroll
