@@ -82,6 +82,15 @@ __device__ __forceinline__ wh4 lds_tr4(const char * a) {
     return __builtin_bit_cast(wh4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_w4) a));
 }
 
+// LDS-DMA of 16 bytes a lane, from base + off (a lane's) + soff to LDS `to` + 16 lane. The buffer form: the compiler
+// counts it with the vector loads alone; behind the global form, which it takes for a flat access, every wait for an
+// LDS read becomes a wait for all of them
+struct FwSrc { __amdgpu_buffer_rsrc_t r; };
+__device__ __forceinline__ FwSrc fw_src(const char * base) { return FwSrc{__builtin_amdgcn_make_buffer_rsrc((void *) base, 0, -1, 0x00027000)}; }
+__device__ __forceinline__ void fw_dma(const FwSrc & s, int off, int soff, char * to) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(s.r, (lds_dma) to, 16, off, soff, 0, 0);
+}
+
 template <int N> __device__ __forceinline__ void fw_vmcnt() {   // at most N vector memory operations outstanding
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
 }
@@ -407,11 +416,12 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
     // ---- staging. f16: instruction x of a tile fills rows 8 (x & 3) .. + 7 of piece x >> 2; lane l brings
     // the chunk that belongs at its place, (l % 8) ^ swz(row) of row l / 8
     const int srow = 8 * (wave & 3) + (lane >> 3), ssrc = 16 * ((lane & 7) ^ fw_swz(srow));
-    auto dma_row = [&](int tile) { return j.kb + (size_t) min((tile & 0x3FFFFFFF) * FW_KT + srow, p.n_kv - 1) * p.k1 + ssrc; };
+    auto dma_off = [&](int tile) { return min(srow, p.n_kv - 1 - (tile & 0x3FFFFFFF) * FW_KT) * (int) p.k1 + ssrc; };
+    auto dma_src = [&](int tile) { return fw_src(j.kb + (size_t) ((tile & 0x3FFFFFFF) * FW_KT) * p.k1); };
     // instruction i of a wave: it keeps to one row group (wave & 3); of eight waves, two share one and halve its pieces
-    auto dma = [&](const char * kr, char * buf, int i) __attribute__((always_inline)) {
+    auto dma = [&](const FwSrc & src, int off, char * buf, int i) __attribute__((always_inline)) {
         const int piece = NW == 8 ? min(2 * i + (wave >> 2), 8) : i;        // (piece 8 is brought twice)
-        __builtin_amdgcn_global_load_lds(kr + 128 * piece, (lds_dma) (buf + piece * FW_PIECE + 1024 * (wave & 3)), 16, 0, 0);
+        fw_dma(src, off, 128 * piece, buf + piece * FW_PIECE + 1024 * (wave & 3));
     };
     // quantised: TPR threads a row take blocks tid % TPR + TPR i through registers
     constexpr int TPR = geo::NT / 32, QI = (18 + TPR - 1) / TPR, QB = qsize_of<QUANT ? KV : GGML_TYPE_Q8_0>();
@@ -494,9 +504,10 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
             for (int i = 0; i < QI; ++i) store(ring[c], i);
             store_top(c);
         } else {
-            const char * kr = dma_row(id[c]);
+            const FwSrc src = dma_src(id[c]);
+            const int off = dma_off(id[c]);
 #pragma unroll
-            for (int i = 0; i < geo::DMA; ++i) dma(kr, ring[c], i);
+            for (int i = 0; i < geo::DMA; ++i) dma(src, off, ring[c], i);
         }
     }
     id[RING - 1] = id[RING - 2] >= 0 ? tiles.next<ROWS>(p, j) : -1;         // fetched by the first body
@@ -551,12 +562,13 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
     // hand, whose values lie in `vbuf`
     // and a further tile goes to `fbuf`: instruction by instruction here, where the matrix unit hides them (all at once
     // behind the barrier they took 800 cycles). They run on past the last tile, into places no longer read
-    auto scores = [&](const char * buf, const char * vbuf, char * fbuf, const char * fsrc, auto with) __attribute__((always_inline)) {
+    auto scores = [&](const char * buf, const char * vbuf, char * fbuf, const FwSrc & fsrc, int foff, auto with) __attribute__((always_inline)) {
         constexpr bool W = decltype(with)::value;
         t[0] = t[1] = wf4{0.f, 0.f, 0.f, 0.f};
+        wf4 tl[2] = {t[0], t[0]};                               // a chain of its own for the low term
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            if constexpr (W && !QUANT) { if (i < geo::DMA) dma(fsrc, fbuf, i); }
+            if constexpr (W && !QUANT) { if (i < geo::DMA) dma(fsrc, foff, fbuf, i); }
             if constexpr (W && QUANT) { if (i % 3 == 0 && i / 3 < QI) store(fbuf, i / 3); }
             if (i + AK < NS) lda(buf, i + AK);
             if (W && i >= NS - AV) ldv(vbuf, i - (NS - AV));
@@ -564,7 +576,7 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
 #pragma unroll
                 for (int u = 0; u < 2; ++u) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], t[u], 0, 0, 0);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], t[u], 0, 0, 0);
+                for (int u = 0; u < 2; ++u) tl[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], tl[u], 0, 0, 0);
             } else {
                 // one 32-block a step: its products are whole, then take the block's step
                 wf4 x[2];
@@ -588,6 +600,7 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (!QUANT) { t[0] += tl[0]; t[1] += tl[1]; }
         exch[par][wave][0][lane] = t[0];
         exch[par][wave][1][lane] = t[1];
     };
@@ -648,9 +661,8 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
     // frees slot C (and tells that the tile after the next is whole)
     auto body = [&](auto slot_) __attribute__((always_inline)) {
         constexpr int C = decltype(slot_)::value, C1 = (C + 1) % RING, F = (C + RING - 1) % RING;
-        const char * fsrc = nullptr;
-        if constexpr (!QUANT) fsrc = dma_row(id[F] >= 0 ? id[F] : id[C]);
-        scores(ring[C1], ring[C], ring[F], fsrc, std::true_type{});
+        const int further = id[F] >= 0 ? id[F] : id[C];         // (behind the last tile: any, into a place no longer read)
+        scores(ring[C1], ring[C], ring[F], dma_src(further), dma_off(further), std::true_type{});
         if constexpr (QUANT) {
             store_top(F);
             load(held >= 0 ? held : id[C]);
@@ -669,7 +681,7 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
     __syncthreads();
     if (id[0] >= 0) {
         ahead(t0);
-        scores(t0, t0, nullptr, nullptr, std::false_type{});
+        scores(t0, t0, nullptr, dma_src(id[0]), 0, std::false_type{});
         fw_barrier();
         whole(id[0], 0, t1);
         const char * last;
@@ -729,14 +741,14 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     tiles.window<ROWS>(p, j);
     const int srow = lane >> 3, ssrc = 16 * ((lane & 7) ^ fw_swz(8 * wave + srow));   // (W is even: the same for rb below)
     auto dma = [&](int tile, char * buf) {
+        const int key0 = (tile & 0x3FFFFFFF) * FW_KT;
+        const FwSrc ks = fw_src(j.kb + (size_t) key0 * p.k1), vs = fw_src(vb + (size_t) key0 * p.v1);
 #pragma unroll
         for (int b = 0; b < 4 / W; ++b) {
-            const int rb = wave + W * b;                        // eight rows
-            const size_t key = (size_t) min((tile & 0x3FFFFFFF) * FW_KT + 8 * rb + srow, p.n_kv - 1);
-            const char * kr = j.kb + key * p.k1 + ssrc, * vr = vb + key * p.v1 + ssrc;
+            const int rb = wave + W * b, row = min(8 * rb + srow, p.n_kv - 1 - key0);   // eight rows
+            const int ko = row * (int) p.k1 + ssrc, vo = row * (int) p.v1 + ssrc;
 #pragma unroll
-            for (int i = 0; i < 5; ++i)
-                __builtin_amdgcn_global_load_lds(i < 3 ? kr + 128 * i : vr + 128 * (i - 3), (lds_dma) (buf + i * FW_PIECE + 1024 * rb), 16, 0, 0);
+            for (int i = 0; i < 5; ++i) fw_dma(i < 3 ? ks : vs, i < 3 ? ko : vo, 128 * (i < 3 ? i : i - 3), buf + i * FW_PIECE + 1024 * rb);
         }
     };
     char * const ring[3] = {t0, t1, t2};
@@ -974,7 +986,8 @@ bool fa_wide_supported(const ggml_tensor * dst) {
               q->ne[2] % m->ne[2] || q->ne[3] % m->ne[3] || m->nb[1] % 2 || m->nb[2] % 2 || m->nb[3] % 2)) return false;
     if (sk && (sk->type != GGML_TYPE_F32 || sk->nb[0] != 4 || sk->ne[0] < q->ne[2])) return false;
     if (mx_op_param<float>(dst, 1) > 0.0f && !m) return false;
-    // grid and index ranges of the kernels
+    // grid and index ranges of the kernels; a tile's rows are addressed in 31 bits
+    if (k->nb[1] > INT32_MAX / 64 || v->nb[1] > INT32_MAX / 64) return false;
     const int64_t G = q->ne[2] / k->ne[2];
     return k->ne[1] <= INT32_MAX / 2 - 64 && q->ne[1] * G < INT32_MAX / 2 && q->ne[1] * q->ne[2] * q->ne[3] < INT32_MAX / 2 &&
            mx_ceil_div(q->ne[1], FW_TB) < 65536 && q->ne[3] < 65536;
