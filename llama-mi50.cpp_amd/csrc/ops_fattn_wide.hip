@@ -201,36 +201,36 @@ struct FwTiles {
     }
 };
 
-// this lane's query row r, channels 32 (s0 + s) + 8 g4 .. + 7 of step s, as two f16 terms: scaled by a
-// power of two that takes the row's largest magnitude to 2^13 .. 2^14 (what the low term then loses is
-// below 2^-38 of it). Returns the scale of its scores. The row is read twice rather than held.
-template <int DK, int NS>
-__device__ __forceinline__ float fw_query(const FwArgs & p, const FwJob & j, int r, int s0, wh8 (&qh)[NS], wh8 (&ql)[NS]) {
+// this lane's query row r, channels 32 (s0 + s) + 8 g4 .. + 7 of step s: fetched first, ...
+template <int NS>
+__device__ __forceinline__ void fw_query(const FwArgs & p, const FwJob & j, int r, int s0, float (&x)[NS][8]) {
     const int g4 = (threadIdx.x & 63) >> 4;
-    const char * qp = p.q + (size_t) (r / p.G) * p.q1 + (size_t) j.head(p, r) * p.q2 + (size_t) j.seq * p.q3 + 32 * g4;
-    float top = 0.f;
-#pragma unroll
-    for (int s = 0; s < DK / 32; ++s) {
-        const uint4 a = ldu16(qp + 128 * s), b = ldu16(qp + 128 * s + 16);
-        float x[8];
-        __builtin_memcpy(&x[0], &a, 16);
-        __builtin_memcpy(&x[4], &b, 16);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-    }
-    top = fw_row4<false>(top);
-    const int e = top > 0.f && top < INFINITY ? max(-100, min(100, 14 - __builtin_amdgcn_frexp_expf(top))) : 0;
-    qp += 128 * s0;
-    asm volatile("" : "+v"(qp));
+    const char * qp = p.q + (size_t) (r / p.G) * p.q1 + (size_t) j.head(p, r) * p.q2 + (size_t) j.seq * p.q3 + 128 * s0 + 32 * g4;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
         const uint4 a = ldu16(qp + 128 * s), b = ldu16(qp + 128 * s + 16);
-        float x[8];
-        __builtin_memcpy(&x[0], &a, 16);
-        __builtin_memcpy(&x[4], &b, 16);
+        __builtin_memcpy(&x[s][0], &a, 16);
+        __builtin_memcpy(&x[s][4], &b, 16);
+    }
+}
+// ... then taken as two f16 terms, scaled by a power of two that takes the largest magnitude of these channels to
+// 2^13 .. 2^14 (what the low term then loses is below 2^-38 of it). Returns the scale of their scores
+template <int NS>
+__device__ __forceinline__ float fw_terms(const FwArgs & p, const float (&x)[NS][8], wh8 (&qh)[NS], wh8 (&ql)[NS]) {
+    float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], e);
-        split8(x, qh[s], ql[s]);
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[s][i]));
+    top = fw_row4<false>(top);
+    const int e = top > 0.f && top < INFINITY ? max(-100, min(100, 14 - __builtin_amdgcn_frexp_expf(top))) : 0;
+    const float f = __builtin_amdgcn_ldexpf(1.f, e);            // (exact: a product that leaves f32's normal range is below the bound)
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[s][i] * f;
+        split8(y, qh[s], ql[s]);
     }
     return p.scale * __builtin_amdgcn_ldexpf(1.f, -e);
 }
@@ -409,6 +409,8 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
     const FwJob j = fw_job<ROWS>(p);
     const int r = min(j.r0 + 16 * rg + n16, j.nrow - 1);        // this lane's row
 
+    float qx[NS][8];
+    fw_query<NS>(p, j, r, NS * dh, qx);                         // (on its way while the tiles are listed)
     FwTiles tiles;
     tiles.w0 = 0;
     tiles.window<ROWS>(p, j);
@@ -515,7 +517,7 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
         if (id[RING - 1] >= 0) { load(id[RING - 1]); held = tiles.next<ROWS>(p, j); }
     }
     wh8 qh[NS], ql[NS];
-    const float qsc = fw_query<576, NS>(p, j, r, NS * dh, qh, ql);
+    const float qsc = fw_terms<NS>(p, qx, qh, ql);              // of this half's part of the scores
 
     wf4 o[ND];
     float m = -INFINITY, l = 0.f;
@@ -601,6 +603,8 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (!QUANT) { t[0] += tl[0]; t[1] += tl[1]; }
+        t[0] *= qsc;
+        t[1] *= qsc;
         exch[par][wave][0][lane] = t[0];
         exch[par][wave][1][lane] = t[1];
     };
@@ -613,8 +617,6 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
         s[0] = t[0] + x0;
         s[1] = t[1] + x1;
         par ^= 1;
-        s[0] *= qsc;
-        s[1] *= qsc;
         if (p.softcap != 0.0f) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = p.softcap * tanhf(s[i >> 2][i & 3]);
@@ -736,6 +738,9 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     const char * const vb = p.v + (size_t) j.hk * p.v2 + (size_t) j.seq * p.v3;
     const int rg0 = j.r0 + 16 * NT * wave;
 
+    float qx[NT][NS][8];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) fw_query<NS>(p, j, min(rg0 + 16 * nt + n16, j.nrow - 1), 0, qx[nt]);
     FwTiles tiles;
     tiles.w0 = 0;
     tiles.window<ROWS>(p, j);
@@ -764,7 +769,7 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     wf4 o[NT][ND];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        qsc[nt] = fw_query<192, NS>(p, j, min(rg0 + 16 * nt + n16, j.nrow - 1), 0, qh[nt], ql[nt]);
+        qsc[nt] = fw_terms<NS>(p, qx[nt], qh[nt], ql[nt]);
         m[nt] = -INFINITY; l[nt] = 0.f;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[nt][d] = wf4{0.f, 0.f, 0.f, 0.f};
@@ -862,43 +867,50 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     for (int nt = 0; nt < NT; ++nt) fw_store<192, 128, GGML_TYPE_F16, ND>(p, j, vb, p.v1, 0, rg0 + 16 * nt, 0, m[nt], l[nt], o[nt]);
 }
 
-// Joins the splits of one row: a workgroup takes 64 output channels of a row, four waves every fourth
-// split. The partials come from L2 / Infinity Cache; the launch is a few microseconds of latency.
+// Joins the splits of one row. A workgroup takes CH channels, four of them a lane; its lane groups (waves) take every
+// GR-th split, so eight loads of 16 bytes a lane are in flight. The partials come from L2 / Infinity Cache.
 template <int DV>
 __global__ __launch_bounds__(256) void k_fattn_wide_join(FwArgs p) {
+    constexpr int CH = DV < 256 ? DV : 256, LG = CH / 4, GR = 256 / LG;     // channels, lanes and groups of them
     __shared__ float wgt[FW_MAX_SPLIT];
-    __shared__ float red[16], part[4][64];
+    __shared__ float red[16];
+    __shared__ __align__(16) wf4 part[GR][LG];
     const int tid = threadIdx.x;
     const size_t rows = (size_t) p.S * p.n_q * p.H, id = blockIdx.x;
     const int h = (int) (id % p.H);
-    float m = -INFINITY;
-    for (int s = tid; s < p.nsplit; s += 256) m = fmaxf(m, p.mpart[s * rows + id]);
-    m = block_max(m, red);
+    float ms = -INFINITY, ls = 0.f;                             // a thread a split
+    if (tid < p.nsplit) { ms = p.mpart[tid * rows + id]; ls = p.lpart[tid * rows + id]; }
+    float m = block_max(ms, red);
     if (p.sinks) m = fmaxf(m, p.sinks[h]);
-    float l = 0.f;
-    for (int s = tid; s < p.nsplit; s += 256) {
-        const float ms = p.mpart[s * rows + id], ls = p.lpart[s * rows + id];
-        const bool none = ms == -INFINITY && ls == 0.f;
-        const float a = none ? 0.f : ms == m ? 1.f : __builtin_amdgcn_exp2f((ms - m) * FW_L2E);
-        wgt[s] = none ? -1.f : a;
-        l += ls * a;
-    }
-    __syncthreads();
-    l = block_sum(l, red);
+    const bool none = ms == -INFINITY && ls == 0.f;             // a split that saw nothing left nothing to read
+    const float w = none ? 0.f : ms == m ? 1.f : __builtin_amdgcn_exp2f((ms - m) * FW_L2E);
+    wgt[tid] = none ? -1.f : w;
+    float l = block_sum(ls * w, red);
     if (p.sinks) l += __builtin_amdgcn_exp2f((p.sinks[h] - m) * FW_L2E);
-    const int c = blockIdx.y * 64 + (tid & 63), w = tid >> 6;
-    float o = 0.f;
-#pragma unroll 4
-    for (int s = w; s < p.nsplit; s += 4) {
-        const float a = wgt[s];
-        if (!(a < 0.f)) o += a * p.opart[(s * rows + id) * DV + c];
-    }
-    part[w][tid & 63] = o;
     __syncthreads();
-    if (w) return;
-    o = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+    const int c = tid % LG, g = tid / LG;
+    const float * src = p.opart + id * DV + blockIdx.y * CH + 4 * c;
+    wf4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = g; s0 < p.nsplit; s0 += 8 * GR) {
+        wf4 v[8];
+        float a[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int s = s0 + i * GR;
+            a[i] = s < p.nsplit ? wgt[s] : -1.f;
+            v[i] = a[i] < 0.f ? wf4{0.f, 0.f, 0.f, 0.f} : *(const wf4 *) (src + (size_t) s * rows * DV);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (!(a[i] < 0.f)) o += v[i] * a[i];
+    }
+    part[g][c] = o;
+    __syncthreads();
+    if (g) return;
+#pragma unroll
+    for (int i = 1; i < GR; ++i) o += part[i][c];
     const size_t t = id / p.H % p.n_q, seq = id / ((size_t) p.H * p.n_q);
-    ((float *) (p.dst + (size_t) h * p.d1 + t * p.d2 + seq * p.d3))[c] = l == 0.f ? 0.f : o / l;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *(wf4 *) (p.dst + (size_t) h * p.d1 + t * p.d2 + seq * p.d3 + 4 * (blockIdx.y * CH + 4 * c)) = o * inv;
 }
 
 // The mask's tile map: for 32 tokens x one key tile, whether some key is visible and whether some value
@@ -1044,7 +1056,7 @@ void fa_wide_run(OpCtx & c, ggml_tensor * dst) {
     else FL(GGML_TYPE_Q4_0);
 #undef FL
     if (pl.nsplit > 1) {
-        const dim3 grid((unsigned) (a.S * a.n_q * a.H), (unsigned) (DV / 64));
+        const dim3 grid((unsigned) (a.S * a.n_q * a.H), (unsigned) (DV / std::min(DV, 256)));
         if (pl.wide) k_fattn_wide_join<512><<<grid, 256, 0, c.st>>>(a);
         else         k_fattn_wide_join<128><<<grid, 256, 0, c.st>>>(a);
     }
