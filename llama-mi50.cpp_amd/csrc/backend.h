@@ -93,6 +93,7 @@ struct GraphCache {
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
     int hits = 0;
+    bool eager = false;           // few nodes: run as they are (kEagerNodes, exec.cpp), never captured
     uint64_t last_use = 0;        // LRU among the stream's slots
 };
 constexpr int kGraphSlots = 8;    // captured cgraphs kept per stream (a pp2048 prompt: 4 ubatch shapes)

@@ -855,6 +855,11 @@ void stream_reserve_node(Stream * s, const ggml_tensor * n) {
     stream_reserve(s, scratch_bytes(n), slot, mmq_act_bytes(n));
 }
 
+// A graph of so few nodes (a fused group counts as one) is run as it is: launching a capture costs the host 16 us
+// before the first kernel, a launch some 3 us. Measured back to back (chains of SCALE, us a pass, replayed / run):
+// 1 launch 15.9 / 3.3, 2 16.6 / 6.2, 4 16.9 / 11.6, 6 17.7 / 21.1, 8 21.0 / 27.2; a node is one to three launches
+constexpr uint64_t kEagerNodes = 3;
+
 // A node whose kernel checks nothing further and that supports_op refuses: the graph fails as a
 // whole (GGML_STATUS_FAILED) instead of reading or writing out of range
 static bool node_refused(const ggml_tensor * n) {
@@ -904,6 +909,7 @@ void graph_compute_impl(Stream * s, ggml_cgraph * g, ggml_status * status) {
             GraphCache & gc = s->gslots[k];
             s->gcur = k;
             gc.last_use = ++s->gtick;
+            if (gc.eager) { run_nodes(s, g); return; }
             if (gc.exec && gc.buf_gen == g_buf_gen.load()) {
                 HIP_CHECK(hipGraphLaunch(gc.exec, s->stream));
                 s->us_launch += std::chrono::duration<double, std::micro>(std::chrono::steady_clock::now() - t1).count();
@@ -926,6 +932,7 @@ void graph_compute_impl(Stream * s, ggml_cgraph * g, ggml_status * status) {
             if (gc.graph) { HIP_CHECK(hipGraphDestroy(gc.graph)); gc.graph = nullptr; }
             gc.key = s->gsig;
             gc.hits = 0;
+            gc.eager = false;
             gc.last_use = ++s->gtick;
             s->gcur = v;
         }
@@ -979,7 +986,9 @@ void graph_compute_impl(Stream * s, ggml_cgraph * g, ggml_status * status) {
         // (the changing ubatch shapes of a long prompt, one-off graphs) would pay the capture
         // and evict a graph that does repeat; there the capture waits for a second sighting.
         static const bool second = getenv("GGML_MI355X_CAPTURE_SECOND") != nullptr;
+        const uint64_t run0 = s->n_nodes_run, fused0 = s->n_fused;
         run_nodes(s, g);
+        if (!split && s->n_nodes_run - run0 - (s->n_fused - fused0) <= kEagerNodes) { gc.eager = true; return; }
         if (second || evicted) { s->split_graph = false; return; }
         HIP_CHECK(hipStreamBeginCapture(s->stream, hipStreamCaptureModeThreadLocal));
         // (the kernel-choice log and the executor counters record the eager pass only: the
