@@ -48,29 +48,37 @@ __global__ __launch_bounds__(256) void k_rope_axes(const char * __restrict__ x, 
                                                    char * __restrict__ y, G4 gx, G4 gy, RopeP p, int np, int hper) {
     __shared__ float2 tab[MX_ROPE_MAXP];
     const int64_t i2 = blockIdx.x % gx.ne[2], i3 = blockIdx.x / gx.ne[2];
-    for (int i = threadIdx.x; i < np; i += blockDim.x) tab[i] = rope_pair(p, i, pos, i2, gx.ne[2], ff);
-    __syncthreads();
     const char * px = x + i2 * gx.nb[2] + i3 * gx.nb[3];
     char * py = y + i2 * gy.nb[2] + i3 * gy.nb[3];
     const int h0 = blockIdx.y * hper, nh = min(hper, (int) gx.ne[1] - h0);
-    const int steps = np / V;                                   // a head's pairs, V at a time
-    for (int u = threadIdx.x; u < nh * steps; u += blockDim.x) {
+    const int steps = np / V, n = nh * steps;                   // a head's pairs, V at a time
+    Pack<T, V> lo, hi;
+    auto fetch = [&](int u) {                                   // on its way while the table, or the step before, is computed
+        const T * rx = (const T *) (px + (h0 + u / steps) * gx.nb[1]);
+        const int i = u % steps * V;
+        lo = ldv<T, V>(rx + (ADJ ? 2 * i : i));
+        hi = ldv<T, V>(rx + (ADJ ? 2 * i + V : i + np));
+    };
+    if (threadIdx.x < n) fetch(threadIdx.x);
+    for (int i = threadIdx.x; i < np; i += blockDim.x) tab[i] = rope_pair(p, i, pos, i2, gx.ne[2], ff);
+    __syncthreads();
+    for (int u = threadIdx.x; u < n; u += blockDim.x) {
         const int h = h0 + u / steps, i = u % steps * V;
-        const T * rx = (const T *) (px + h * gx.nb[1]);
         T * ry = (T *) (py + h * gy.nb[1]);
-        Pack<T, V> lo = ldv<T, V>(rx + (ADJ ? 2 * i : i)), hi = ldv<T, V>(rx + (ADJ ? 2 * i + V : i + np));
+        Pack<T, V> alo = lo, ahi = hi;
+        if (u + (int) blockDim.x < n) fetch(u + blockDim.x);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             // (ADJ: pair j is elements 2j and 2j + 1 of the 2V that lo and hi hold; V = 1: lo and hi)
-            T & a = !ADJ ? lo.v[j] : (2 * j < V ? lo.v[(2 * j) % V] : hi.v[(2 * j) % V]);
-            T & b = !ADJ || V == 1 ? hi.v[j] : (2 * j < V ? lo.v[(2 * j + 1) % V] : hi.v[(2 * j + 1) % V]);
+            T & a = !ADJ ? alo.v[j] : (2 * j < V ? alo.v[(2 * j) % V] : ahi.v[(2 * j) % V]);
+            T & b = !ADJ || V == 1 ? ahi.v[j] : (2 * j < V ? alo.v[(2 * j + 1) % V] : ahi.v[(2 * j + 1) % V]);
             const float2 t = tab[i + j];
             const float x0 = rd<T>(a), x1 = rd<T>(b);
             a = wr<T>(x0 * t.x - x1 * t.y);
             b = wr<T>(x0 * t.y + x1 * t.x);
         }
-        stv<T, V>(ry + (ADJ ? 2 * i : i), lo);
-        stv<T, V>(ry + (ADJ ? 2 * i + V : i + np), hi);
+        stv<T, V>(ry + (ADJ ? 2 * i : i), alo);
+        stv<T, V>(ry + (ADJ ? 2 * i + V : i + np), ahi);
     }
     const int rest = (int) gx.ne[0] - 2 * np;                   // channels that do not turn
     for (int u = threadIdx.x; u < nh * rest; u += blockDim.x) {
@@ -221,10 +229,14 @@ struct AppendP {
 };
 constexpr int APPEND_MAX_ROW = 8192;                            // elements of both rows in LDS: 32 KB
 
-// `row` (LDS, width values) -> cell idx[t]; a cell outside the cache takes nothing
-__device__ __forceinline__ void store_row(const RowDst & d, const float * row, int64_t t) {
-    const int64_t cell = d.i64 ? *(const int64_t *) (d.idx + t * d.idx_nb) : (int64_t) *(const int32_t *) (d.idx + t * d.idx_nb);
-    if (cell < 0 || cell >= d.ne1) return;
+// the cell of token t, -1 when it is none of the cache's
+__device__ __forceinline__ int64_t cell_of(const RowDst & d, int64_t t) {
+    const int64_t c = d.i64 ? *(const int64_t *) (d.idx + t * d.idx_nb) : (int64_t) *(const int32_t *) (d.idx + t * d.idx_nb);
+    return c < 0 || c >= d.ne1 ? -1 : c;
+}
+// `row` (LDS, width values) -> that cell; none takes nothing
+__device__ __forceinline__ void store_row(const RowDst & d, const float * row, int64_t cell) {
+    if (cell < 0) return;
     char * o = d.base + cell * d.nb1;
     const int nt = blockDim.x;
     switch (d.type) {                                           // uniform
@@ -262,48 +274,71 @@ __global__ __launch_bounds__(256) void k_append_rows(AppendP p) {
     __shared__ float2 tab[MX_ROPE_MAXP];
     __shared__ float red[16];
     const int64_t t = blockIdx.x;
-    const int nt = blockDim.x;
-    for (int i = threadIdx.x; i < p.np; i += nt) tab[i] = rope_pair(p.rope, i, p.pos, t, p.ntok, p.ff);
+    const int nt = blockDim.x, tid = threadIdx.x;
+    // everything the row needs is fetched first, up to AHEAD elements (pairs) a thread; a chain of table, sum and
+    // rotation that fetched its own spent 9 us on 2011 latent rows, 7 of them waiting
+    constexpr int AHEAD = 4;
+    float nv[AHEAD], vv[AHEAD], r0[AHEAD], r1[AHEAD];
+    const float * xn = (const float *) (p.nx + t * p.n_tok), * xv = (const float *) (p.vx + t * p.v_tok);
+    const int pairs = p.heads * p.np;
+    auto pair = [&](int u, float & x0, float & x1) {
+        const int h = u / p.np, i = u % p.np;
+        const float * x = (const float *) (p.rx + t * p.r_tok + h * p.r_head);
+        x0 = x[p.adj ? 2 * i : i];
+        x1 = x[p.adj ? 2 * i + 1 : i + p.np];
+    };
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+        const int i = tid + a * nt;
+        nv[a] = i < p.n_norm ? xn[i] : 0.f;
+        vv[a] = i < p.v.width ? xv[i] : 0.f;
+        if (i < pairs) pair(i, r0[a], r1[a]);
+    }
+    const int64_t kcell = cell_of(p.k, t), vcell = p.v.width ? cell_of(p.v, t) : -1;
+    for (int i = tid; i < p.np; i += nt) tab[i] = rope_pair(p.rope, i, p.pos, t, p.ntok, p.ff);
     if (p.n_norm) {
-        const float * x = (const float *) (p.nx + t * p.n_tok);
         float s = 0.f;
-        for (int i = threadIdx.x; i < p.n_norm; i += nt) {
-            const float v = x[i];
-            row[p.norm_at + i] = v;
-            s += v * v;
-        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) s += nv[a] * nv[a];
+        for (int i = tid + AHEAD * nt; i < p.n_norm; i += nt) s += xn[i] * xn[i];
         s = block_sum(s, red);
         const float inv = 1.0f / sqrtf(s / p.n_norm + p.eps);
         float * out = p.nout ? (float *) (p.nout + t * p.nout_tok) : nullptr;
-        for (int i = threadIdx.x; i < p.n_norm; i += nt) {      // the values this thread left above
-            const float v = row[p.norm_at + i] * inv * p.nw[i];
+        auto put = [&](int i, float x) {
+            const float v = x * inv * p.nw[i];
             row[p.norm_at + i] = v;
             if (out) out[i] = v;
-        }
+        };
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) if (tid + a * nt < p.n_norm) put(tid + a * nt, nv[a]);
+        for (int i = tid + AHEAD * nt; i < p.n_norm; i += nt) put(i, xn[i]);
     }
-    if (p.v.width) {
-        const float * x = (const float *) (p.vx + t * p.v_tok);
-        for (int i = threadIdx.x; i < p.v.width; i += nt) row[v0 + i] = x[i];
-    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) if (tid + a * nt < p.v.width) row[v0 + tid + a * nt] = vv[a];
+    for (int i = tid + AHEAD * nt; i < p.v.width; i += nt) row[v0 + i] = xv[i];
     __syncthreads();                                            // the table
-    const int rest = p.dim - 2 * p.np;
-    for (int u = threadIdx.x; u < p.heads * p.np; u += nt) {
+    auto turn = [&](int u, float x0, float x1) {
         const int h = u / p.np, i = u % p.np;
-        const float * x = (const float *) (p.rx + t * p.r_tok + h * p.r_head);
-        const int a = p.adj ? 2 * i : i, b = p.adj ? 2 * i + 1 : i + p.np;
         const float2 cs = tab[i];
-        const float x0 = x[a], x1 = x[b];
         float * r = row + p.rot_at + h * p.dim;
-        r[a] = x0 * cs.x - x1 * cs.y;
-        r[b] = x0 * cs.y + x1 * cs.x;
+        r[p.adj ? 2 * i : i] = x0 * cs.x - x1 * cs.y;
+        r[p.adj ? 2 * i + 1 : i + p.np] = x0 * cs.y + x1 * cs.x;
+    };
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) if (tid + a * nt < pairs) turn(tid + a * nt, r0[a], r1[a]);
+    for (int u = tid + AHEAD * nt; u < pairs; u += nt) {
+        float x0, x1;
+        pair(u, x0, x1);
+        turn(u, x0, x1);
     }
-    for (int u = threadIdx.x; u < p.heads * rest; u += nt) {
+    const int rest = p.dim - 2 * p.np;
+    for (int u = tid; u < p.heads * rest; u += nt) {
         const int h = u / rest, i = 2 * p.np + u % rest;
         row[p.rot_at + h * p.dim + i] = ((const float *) (p.rx + t * p.r_tok + h * p.r_head))[i];
     }
     __syncthreads();
-    store_row(p.k, row, t);
-    if (p.v.width) store_row(p.v, row + v0, t);
+    store_row(p.k, row, kcell);
+    store_row(p.v, row + v0, vcell);
 }
 
 static const ggml_tensor * through_views(const ggml_tensor * t) {
