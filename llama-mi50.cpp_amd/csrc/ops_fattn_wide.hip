@@ -67,6 +67,13 @@ __device__ __forceinline__ void split2(float x0, float x1, int j, wh8 & hi, wh8 
     hi[j] = h[0]; hi[j + 1] = h[1];
     lo[j] = l[0]; lo[j + 1] = l[1];
 }
+// the same of the products x0 d0, x1 d1: the remainder of the whole product
+__device__ __forceinline__ void split2p(float x0, float d0, float x1, float d1, int j, wh8 & hi, wh8 & lo) {
+    const wh2 h = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(x0, d0, 0.f), __builtin_fmaf(x1, d1, 0.f)));   // (d f16: mixed FMAs)
+    const wh2 l = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(x0, d0, -(float) h[0]), __builtin_fmaf(x1, d1, -(float) h[1])));
+    hi[j] = h[0]; hi[j + 1] = h[1];
+    lo[j] = l[0]; lo[j + 1] = l[1];
+}
 __device__ __forceinline__ void split8(const float (&x)[8], wh8 & hi, wh8 & lo) {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) split2(x[j], x[j + 1], j, hi, lo);
@@ -130,14 +137,17 @@ struct FwJob {
 };
 
 // (KV head, sequence) units: with a multiple of eight the workgroups of one unit stay on one XCD and
-// share its L2; the last rows (most keys, under a causal mask) go first
-template <int ROWS> __device__ __forceinline__ FwJob fw_job(const FwArgs & p) {
+// share its L2; the last rows (most keys, under a causal mask) go first. FOLD, two workgroups a CU: those
+// that take the second places of an XCD's 32 CUs run the other way, so that the last rows share a CU with
+// the first ones
+template <int ROWS, bool FOLD> __device__ __forceinline__ FwJob fw_job(const FwArgs & p) {
     FwJob j;
     j.nrow = p.n_q * p.G;
     const int nrb = (j.nrow + ROWS - 1) / ROWS, units = p.Hkv * p.S;
     int unit, rb;
-    if (units % 8 == 0) { unit = blockIdx.x % 8 + 8 * (blockIdx.x / 8 / nrb); rb = nrb - 1 - blockIdx.x / 8 % nrb; }
-    else { unit = blockIdx.x / nrb; rb = nrb - 1 - blockIdx.x % nrb; }
+    if (units % 8 == 0) { unit = blockIdx.x % 8 + 8 * (blockIdx.x / 8 / nrb); rb = blockIdx.x / 8 % nrb; }
+    else { unit = blockIdx.x / nrb; rb = blockIdx.x % nrb; }
+    if (!FOLD || units % 8 != 0 || gridDim.x > 512 || !(unit / 8 * nrb / 32 & 1)) rb = nrb - 1 - rb;
     j.hk = unit % p.Hkv;
     j.seq = unit / p.Hkv;
     j.r0 = rb * ROWS;
@@ -380,18 +390,115 @@ __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, cons
 // much for one wave beside the rest of it, so the pair shares: wave dh multiplies channels [288 dh, + 288)
 // of the keys, the halves of the scores are exchanged through LDS (the only barrier of a tile), both do
 // the softmax, and each keeps half of the output channels.
+// A quantised cache takes four waves more, one a SIMD, that turn the blocks into f16 integers ahead of the others:
+// done by the same waves it left the matrix unit idle (4 bits 2.6 us a tile instead of 1.8).
 template <int KV, int RG> struct FlGeo {
     static constexpr bool QUANT = KV != GGML_TYPE_F16;
-    static constexpr int NT = 128 * RG;                         // threads
+    static constexpr int NT = 128 * RG + (QUANT ? 256 : 0);     // threads
     // tiles in the ring, three ahead of the one in use where they fit beside the exchange
     static constexpr int RING = !QUANT && RG == 2 ? 4 : 3;
-    static constexpr int STEPS = QUANT ? 18 * FW_KT * 4 : 0;    // the blocks' steps, [block][key] f32
+    static constexpr int STEPS = QUANT ? 18 * FW_KT * 2 : 0;    // the blocks' steps, [block][key] f16
     static constexpr int BUF = 9 * FW_PIECE + STEPS;
     static constexpr int DMA = (36 + 2 * RG - 1) / (2 * RG);    // LDS-DMA instructions of a wave and tile
 };
 
+// The producers of a quantised cache: blocks through registers, two tiles ahead of the store, into the slots of the ring;
+// the same barriers as the kernel below
+template <int KV, int ROWS>
+__device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, char * const (&ring)[3], float (&dtop)[3][4]) {
+    // eight threads a row take two whole 32-blocks each, x and x + 8, and eight values of the last two blocks
+    constexpr int QB = qsize_of<KV>();
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row = tid >> 3, x8 = tid & 7, sw = fw_swz(row), pblk = 16 + (x8 >> 2), pval = 8 * (x8 & 3);
+    struct Regs { uint4 a[2], b[2]; uint2 w; uint16_t d[3]; } set[2];
+    auto load = [&](int tile, Regs & q) __attribute__((always_inline)) {
+        const char * kr = j.kb + (size_t) min((tile & 0x3FFFFFFF) * FW_KT + row, p.n_kv - 1) * p.k1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const char * b = kr + (x8 + 8 * i) * QB;
+            q.d[i] = ld_u16(b);
+            q.a[i] = ldu16(b + 2);
+            if constexpr (KV == GGML_TYPE_Q8_0) q.b[i] = ldu16(b + 18);
+        }
+        const char * b = kr + pblk * QB;
+        q.d[2] = ld_u16(b);
+        __builtin_memcpy(&q.w, b + 2 + (KV == GGML_TYPE_Q8_0 ? pval : pval & 15), 8);
+    };
+    // integers to f16 exactly: 1024 + n has n in its low bits, two at a time. Bytes 2t, 2t + 1 of u (n + 128; n + 8)
+    auto pair = [](uint32_t u, int t) __attribute__((always_inline)) {
+        const _Float16 off = KV == GGML_TYPE_Q8_0 ? 1152.f : 1032.f;
+        const uint32_t pr = __builtin_amdgcn_perm(0x64646464u, u, t ? 0x04030402u : 0x04010400u);
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(wh2, pr) - wh2{off, off});
+    };
+    auto store = [&](const Regs & q, int slot) __attribute__((always_inline)) {
+        char * const buf = ring[slot];
+        uint16_t * const steps = (uint16_t *) (buf + 9 * FW_PIECE);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int b = x8 + 8 * i;
+            uint32_t w[16];                                     // 32 values in order, as f16 pairs
+            if constexpr (KV == GGML_TYPE_Q8_0) {
+                const uint32_t src[8] = {q.a[i].x, q.a[i].y, q.a[i].z, q.a[i].w, q.b[i].x, q.b[i].y, q.b[i].z, q.b[i].w};
+#pragma unroll
+                for (int c = 0; c < 16; ++c) w[c] = pair(src[c >> 1] ^ 0x80808080u, c & 1);
+            } else {
+                const uint32_t src[4] = {q.a[i].x, q.a[i].y, q.a[i].z, q.a[i].w};
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {                   // low nibbles are values 0..15, high 16..31
+                    w[c] = pair(src[c >> 1] & 0x0F0F0F0Fu, c & 1);
+                    w[c + 8] = pair(src[c >> 1] >> 4 & 0x0F0F0F0Fu, c & 1);
+                }
+            }
+            steps[b * FW_KT + row] = q.d[i];
+            char * kd = buf + (b >> 1) * FW_PIECE + 128 * row;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                *(uint4 *) (kd + 16 * ((4 * (b & 1) + c) ^ sw)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const uint32_t u = c < 2 ? q.w.x : q.w.y;
+            w[c] = pair(KV == GGML_TYPE_Q8_0 ? u ^ 0x80808080u : (pval & 16 ? u >> 4 : u) & 0x0F0F0F0Fu, c & 1);
+        }
+        steps[pblk * FW_KT + row] = q.d[2];
+        *(uint4 *) (buf + 8 * FW_PIECE + 128 * row + 16 * ((x8 & 7) ^ sw)) = make_uint4(w[0], w[1], w[2], w[3]);
+        const float top = wave_max<64>(fmaxf(fmaxf(fabsf(h2f(q.d[0])), fabsf(h2f(q.d[1]))), fabsf(h2f(q.d[2]))));
+        if (lane == 0) dtop[slot][wave] = top;
+    };
+
+    FwTiles tiles;
+    tiles.w0 = 0;
+    tiles.window<ROWS>(p, j);
+    // the first two tiles stored, the third and fourth in registers
+    int t0 = tiles.next<ROWS>(p, j), t1 = t0 >= 0 ? tiles.next<ROWS>(p, j) : -1;
+    if (t0 >= 0) load(t0, set[0]);
+    if (t1 >= 0) load(t1, set[1]);
+    int t2 = t1 >= 0 ? tiles.next<ROWS>(p, j) : -1, t3 = t2 >= 0 ? tiles.next<ROWS>(p, j) : -1;
+    if (t0 >= 0) store(set[0], 0);
+    if (t2 >= 0) load(t2, set[0]);
+    if (t1 >= 0) store(set[1], 1);
+    if (t3 >= 0) load(t3, set[1]);
+    fw_barrier();
+    if (t0 < 0) return;
+    fw_barrier();
+    // beside tile i + 1's scores and tile i's values: tile i + 2 to its slot, tile i + 4 on its way
+    auto body = [&](auto i_) __attribute__((always_inline)) {
+        constexpr int I = decltype(i_)::value;
+        if (t1 < 0) return false;
+        if (t2 >= 0) store(set[I & 1], (I + 2) % 3);
+        const int t4 = t3 >= 0 ? tiles.next<ROWS>(p, j) : -1;
+        if (t4 >= 0) load(t4, set[I & 1]);
+        t1 = t2; t2 = t3; t3 = t4;
+        fw_barrier();
+        return true;
+    };
+    while (body(std::integral_constant<int, 0>{}) && body(std::integral_constant<int, 1>{}) && body(std::integral_constant<int, 2>{}) &&
+           body(std::integral_constant<int, 3>{}) && body(std::integral_constant<int, 4>{}) && body(std::integral_constant<int, 5>{})) {}
+}
+
 template <int KV, int RG>
-__global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwArgs p) {
+__global__ __launch_bounds__((FlGeo<KV, RG>::NT), (FlGeo<KV, RG>::NT / 256)) void k_fattn_latent(FwArgs p) {
     using geo = FlGeo<KV, RG>;
     constexpr bool QUANT = geo::QUANT;
     constexpr int RING = geo::RING, NS = 9, ND = 16, ROWS = 16 * RG, NW = 2 * RG;
@@ -401,14 +508,21 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
     __shared__ __align__(128) char t2[geo::BUF];
     __shared__ __align__(128) char t3[RING == 4 ? geo::BUF : 16];
     __shared__ __align__(16) wf4 exch[2][NW][2][64];
-    __shared__ __align__(16) float dtop[QUANT ? 3 : 1][QUANT ? NW : 1];   // the tiles' largest steps, wave by wave
+    __shared__ __align__(16) float dtop[QUANT ? 3 : 1][4];      // the tiles' largest steps, wave by wave
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, g4 = lane >> 4;
     const int rg = wave >> 1, dh = wave & 1;
-    const FwJob j = fw_job<ROWS>(p);
+    const FwJob j = fw_job<ROWS, false>(p);
     const int r = min(j.r0 + 16 * rg + n16, j.nrow - 1);        // this lane's row
 
+    if constexpr (QUANT) {
+        if (wave >= NW) {
+            char * const ring[3] = {t0, t1, t2};
+            fw_produce<KV, ROWS>(p, j, ring, dtop);
+            return;
+        }
+    }
     float qx[NS][8];
     fw_query<NS>(p, j, r, NS * dh, qx);                         // (on its way while the tiles are listed)
     FwTiles tiles;
@@ -425,87 +539,14 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
         const int piece = NW == 8 ? min(2 * i + (wave >> 2), 8) : i;        // (piece 8 is brought twice)
         fw_dma(src, off, 128 * piece, buf + piece * FW_PIECE + 1024 * (wave & 3));
     };
-    // quantised: TPR threads a row take blocks tid % TPR + TPR i through registers
-    constexpr int TPR = geo::NT / 32, QI = (18 + TPR - 1) / TPR, QB = qsize_of<QUANT ? KV : GGML_TYPE_Q8_0>();
-    uint4 qa[QUANT ? QI : 1], qb[KV == GGML_TYPE_Q8_0 ? QI : 1];
-    uint16_t qd[QUANT ? QI : 1];
-    auto load = [&](int tile) {
-        if constexpr (QUANT) {
-            const char * kr = j.kb + (size_t) min((tile & 0x3FFFFFFF) * FW_KT + tid / TPR, p.n_kv - 1) * p.k1;
-#pragma unroll
-            for (int i = 0; i < QI; ++i) {
-                const char * b = kr + min(tid % TPR + TPR * i, 17) * QB;
-                qd[i] = ld_u16(b);
-                qa[i] = ldu16(b + 2);
-                if constexpr (KV == GGML_TYPE_Q8_0) qb[i] = ldu16(b + 18);
-            }
-        }
-    };
-    auto store = [&](char * buf, int i) __attribute__((always_inline)) {      // the thread's block i
-        if constexpr (QUANT) {
-            // integers to f16 exactly: 1024 + n has n in its low bits, two at a time
-            const int row = tid / TPR, sw = fw_swz(row);
-            float * steps = (float *) (buf + 9 * FW_PIECE);
-            {
-                const int b = tid % TPR + TPR * i;
-                if (b < 18) {
-                    steps[b * FW_KT + row] = h2f(qd[i]);
-                    uint32_t w[16];                             // 32 values in order, as f16 pairs
-                    if constexpr (KV == GGML_TYPE_Q8_0) {
-                        const uint32_t src[8] = {qa[i].x, qa[i].y, qa[i].z, qa[i].w, qb[i].x, qb[i].y, qb[i].z, qb[i].w};
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const uint32_t u = src[c] ^ 0x80808080u;            // n + 128
-#pragma unroll
-                            for (int t = 0; t < 2; ++t) {
-                                const uint32_t pr = __builtin_amdgcn_perm(0x64646464u, u, t ? 0x04030402u : 0x04010400u);
-                                w[2 * c + t] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(wh2, pr) - wh2{(_Float16) 1152.f, (_Float16) 1152.f});
-                            }
-                        }
-                    } else {
-                        const uint32_t src[4] = {qa[i].x, qa[i].y, qa[i].z, qa[i].w};
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int t = 0; t < 4; ++t) {       // bytes 4c + 2(t&1), + 1; low nibbles are values 0..15, high 16..31
-                                const uint32_t nib = (t & 2 ? src[c] >> 4 : src[c]) & 0x0F0F0F0Fu;
-                                const uint32_t pr = __builtin_amdgcn_perm(0x64646464u, nib, t & 1 ? 0x04030402u : 0x04010400u);
-                                w[2 * c + (t & 1) + (t & 2 ? 8 : 0)] =
-                                    __builtin_bit_cast(uint32_t, __builtin_bit_cast(wh2, pr) - wh2{(_Float16) 1032.f, (_Float16) 1032.f});
-                            }
-                    }
-                    char * kd = buf + (b >> 1) * FW_PIECE + 128 * row;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        *(uint4 *) (kd + 16 * ((4 * (b & 1) + c) ^ sw)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-                }
-            }
-        }
-    };
-    auto store_top = [&](int slot) __attribute__((always_inline)) {
-        if constexpr (QUANT) {
-            float top = 0.f;
-#pragma unroll
-            for (int i = 0; i < QI; ++i) top = fmaxf(top, fabsf(h2f(qd[i])));   // (blocks past the row's repeat its last)
-            top = wave_max<64>(top);
-            if (lane == 0) dtop[slot][wave] = top;
-        }
-    };
-
-    // ---- the first tiles on their way, then the query rows. id[c]: the tile in slot c of the ring (-1: none);
-    // quantised, `held` is one more in registers
+    // ---- the first tiles on their way, then the query rows. id[c]: the tile in slot c of the ring (-1: none)
     char * const ring[4] = {t0, t1, t2, t3};
-    int id[RING], held = -1;
+    int id[RING];
 #pragma unroll
     for (int c = 0; c < RING - 1; ++c) {
         id[c] = c == 0 || id[c - 1] >= 0 ? tiles.next<ROWS>(p, j) : -1;
-        if (id[c] < 0) continue;
-        if constexpr (QUANT) {
-            load(id[c]);
-#pragma unroll
-            for (int i = 0; i < QI; ++i) store(ring[c], i);
-            store_top(c);
-        } else {
+        if constexpr (!QUANT) {
+            if (id[c] < 0) continue;
             const FwSrc src = dma_src(id[c]);
             const int off = dma_off(id[c]);
 #pragma unroll
@@ -513,9 +554,6 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
         }
     }
     id[RING - 1] = id[RING - 2] >= 0 ? tiles.next<ROWS>(p, j) : -1;         // fetched by the first body
-    if constexpr (QUANT) {
-        if (id[RING - 1] >= 0) { load(id[RING - 1]); held = tiles.next<ROWS>(p, j); }
-    }
     wh8 qh[NS], ql[NS];
     const float qsc = fw_terms<NS>(p, qx, qh, ql);              // of this half's part of the scores
 
@@ -538,15 +576,20 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
     int par = 0;
     wf4 s[2], t[2];                                             // the scores of the tile in hand, this half's of the next
     float ms = 0.f, qf = 1.f;
-    wh8 ph, pl;
+    wh8 ph[QUANT ? 2 : 1], pl[QUANT ? 2 : 1];                   // (quantised: a block's and the next one's)
     float e[8];
     // fragments from LDS are read AK (AV) steps ahead: with eight waves at it a read takes some 250 cycles, a step's
     // matrix instructions 64. The first ones before the barrier's other business, and before the end of the scores
-    constexpr int AK = QUANT && RG == 4 ? 2 : 4, AV = QUANT && RG == 4 ? 2 : 3;
+    constexpr int AK = QUANT ? 2 : 4, AV = QUANT ? 2 : 3;
     wh8 a[AK + 1][2], v[AV + 1][2];
+    wh4 ad[QUANT ? AK + 2 : 1][2], vd[QUANT ? AV + 1 : 1][2];   // quantised: their steps, of the lane's keys
     auto lda = [&](const char * buf, int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) a[i % (AK + 1)][u] = *(const wh8 *) (buf + (i & 1 ? ka1 : ka0) + (i >> 1) * FW_PIECE + 2048 * u);
+        if constexpr (QUANT) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) ad[i % (AK + 2)][u] = *(const wh4 *) (buf + 9 * FW_PIECE + 2 * ((NS * dh + i) * FW_KT + 16 * u + 4 * g4));
+        }
     };
     auto ldv = [&](const char * buf, int b) __attribute__((always_inline)) {
 #pragma unroll
@@ -554,6 +597,18 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
             const char * a_ = buf + va[2 * (b & 1) + c] + (b >> 1) * FW_PIECE;
             const wh4 v0 = lds_tr4(a_), v1 = lds_tr4(a_ + 2048);
             v[b % (AV + 1)][c] = wh8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        }
+        if constexpr (QUANT) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) vd[b % (AV + 1)][u] = *(const wh4 *) (buf + 9 * FW_PIECE + 2 * ((8 * dh + 2 * p.vpiece + b) * FW_KT + 16 * u + 4 * g4));
+        }
+    };
+    // quantised: the weights times V's steps of 32-block b, as two terms
+    auto terms = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const wh4 d = vd[b % (AV + 1)][i >> 2];
+            split2p(e[i], (float) d[i & 3], e[i + 1], (float) d[(i & 3) + 1], i, ph[b & 1], pl[b & 1]);
         }
     };
     auto ahead = [&](const char * buf) __attribute__((always_inline)) {
@@ -568,10 +623,16 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
         constexpr bool W = decltype(with)::value;
         t[0] = t[1] = wf4{0.f, 0.f, 0.f, 0.f};
         wf4 tl[2] = {t[0], t[0]};                               // a chain of its own for the low term
+        wf4 x[2][2];
+        auto step = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) t[u][c] = __builtin_fmaf((float) ad[i % (AK + 2)][u][c], x[i & 1][u][c], t[u][c]);
+        };
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             if constexpr (W && !QUANT) { if (i < geo::DMA) dma(fsrc, foff, fbuf, i); }
-            if constexpr (W && QUANT) { if (i % 3 == 0 && i / 3 < QI) store(fbuf, i / 3); }
             if (i + AK < NS) lda(buf, i + AK);
             if (W && i >= NS - AV) ldv(vbuf, i - (NS - AV));
             if constexpr (!QUANT) {
@@ -580,29 +641,25 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
 #pragma unroll
                 for (int u = 0; u < 2; ++u) tl[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], tl[u], 0, 0, 0);
             } else {
-                // one 32-block a step: its products are whole, then take the block's step
-                wf4 x[2];
+                // one 32-block a step: its products are whole, then, a step later, take the block's step
 #pragma unroll
-                for (int u = 0; u < 2; ++u) x[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], wf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], wf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) x[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], x[u], 0, 0, 0);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const wf4 d = *(const wf4 *) (buf + 9 * FW_PIECE + 4 * ((NS * dh + i) * FW_KT + 16 * u + 4 * g4));
-                    t[u] += d * x[u];
-                }
+                for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], x[i & 1][u], 0, 0, 0);
+                if (i) step(i - 1);
             }
             if constexpr (W) {
                 if (i < 8) {
                     e[i] = fw_weight(s, i, ms);
                     l += e[i];
                     if constexpr (QUANT) e[i] *= qf;
-                    else if (i & 1) split2(e[i - 1], e[i], i - 1, ph, pl);
-                }
+                    else if (i & 1) split2(e[i - 1], e[i], i - 1, ph[0], pl[0]);
+                } else if constexpr (QUANT) terms(0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (!QUANT) { t[0] += tl[0]; t[1] += tl[1]; }
+        else step(NS - 1);
         t[0] *= qsc;
         t[1] *= qsc;
         exch[par][wave][0][lane] = t[0];
@@ -625,7 +682,7 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
         if constexpr (QUANT) {
             float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < NW; ++i) top = fmaxf(top, dtop[C][i]);
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, dtop[C][i]);
             const int x = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : -1000;
             if (x > qe) {                                       // the same in every wave; on the first tiles only
                 const float f = __builtin_amdgcn_ldexpf(1.f, max(qe - x, -200));
@@ -643,18 +700,12 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
 #pragma unroll
         for (int b = 0; b < ND / 2; ++b) {
             if (b + AV < ND / 2) ldv(buf, b + AV);
-            if constexpr (QUANT) {                              // a 32-block of V: its steps enter the weights
-                const float * sp = (const float *) (buf + 9 * FW_PIECE) + (8 * dh + 2 * p.vpiece + b) * FW_KT + 4 * g4;
-                const wf4 d0 = *(const wf4 *) sp, d1 = *(const wf4 *) (sp + 16);
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = e[i] * (i < 4 ? d0[i & 3] : d1[i & 3]);
-                split8(x, ph, pl);
-            }
-            o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], ph, o[2 * b], 0, 0, 0);
-            o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], ph, o[2 * b + 1], 0, 0, 0);
-            o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], pl, o[2 * b], 0, 0, 0);
-            o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], pl, o[2 * b + 1], 0, 0, 0);
+            if constexpr (QUANT) { if (b + 1 < ND / 2) terms(b + 1); }          // a 32-block of V: its steps enter the weights
+            const int w = QUANT ? b & 1 : 0;
+            o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], ph[w], o[2 * b], 0, 0, 0);
+            o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], ph[w], o[2 * b + 1], 0, 0, 0);
+            o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], pl[w], o[2 * b], 0, 0, 0);
+            o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], pl[w], o[2 * b + 1], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -665,17 +716,10 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
         constexpr int C = decltype(slot_)::value, C1 = (C + 1) % RING, F = (C + RING - 1) % RING;
         const int further = id[F] >= 0 ? id[F] : id[C];         // (behind the last tile: any, into a place no longer read)
         scores(ring[C1], ring[C], ring[F], dma_src(further), dma_off(further), std::true_type{});
-        if constexpr (QUANT) {
-            store_top(F);
-            load(held >= 0 ? held : id[C]);
-        }
         values(ring[C]);
         if constexpr (!QUANT) fw_vmcnt<(RING - 3) * geo::DMA>();    // the tile after the next has landed
         fw_barrier();
-        if constexpr (QUANT) {
-            id[C] = held;
-            held = held >= 0 ? tiles.next<ROWS>(p, j) : -1;
-        } else id[C] = id[F] >= 0 ? tiles.next<ROWS>(p, j) : -1;
+        id[C] = id[F] >= 0 ? tiles.next<ROWS>(p, j) : -1;
         whole(id[C1], C1, ring[(C + 2) % RING]);                // (fragments read for nothing where no such tile is left)
     };
 
@@ -708,11 +752,12 @@ __global__ __launch_bounds__(128 * RG, RG == 4 ? 2 : 1) void k_fattn_latent(FwAr
             e[i] = fw_weight(s, i, ms);
             l += e[i];
             if constexpr (QUANT) e[i] *= qf;
-            else if (i & 1) split2(e[i - 1], e[i], i - 1, ph, pl);
+            else if (i & 1) split2(e[i - 1], e[i], i - 1, ph[0], pl[0]);
         }
         if constexpr (!QUANT) fw_vmcnt<0>();                    // no DMA outlives the workgroup's LDS
 #pragma unroll
         for (int b = 0; b < AV; ++b) ldv(last, b);
+        if constexpr (QUANT) terms(0);
         values(last);
     }
     if constexpr (QUANT) {
@@ -734,7 +779,7 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     __shared__ __align__(128) char t2[BUF];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, g4 = lane >> 4;
-    const FwJob j = fw_job<ROWS>(p);
+    const FwJob j = fw_job<ROWS, true>(p);
     const char * const vb = p.v + (size_t) j.hk * p.v2 + (size_t) j.seq * p.v3;
     const int rg0 = j.r0 + 16 * NT * wave;
 
@@ -913,6 +958,54 @@ __global__ __launch_bounds__(256) void k_fattn_wide_join(FwArgs p) {
     *(wf4 *) (p.dst + (size_t) h * p.d1 + t * p.d2 + seq * p.d3 + 4 * (blockIdx.y * CH + 4 * c)) = o * inv;
 }
 
+// The same for many rows: a wave a row and CH channels (of 128 channels, each half of it every other split). A workgroup
+// a row took 44 us for 6400 rows of 512 channels and two splits
+template <int DV>
+__global__ __launch_bounds__(256) void k_fattn_wide_join_rows(FwArgs p) {
+    constexpr int CH = DV < 256 ? DV : 256, LG = CH / 4, GR = 64 / LG;      // lanes of a split's part, splits at a time
+    const int lane = threadIdx.x & 63;
+    const size_t rows = (size_t) p.S * p.n_q * p.H, id = (size_t) blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= rows) return;
+    const int h = (int) (id % p.H);
+    const float sink = p.sinks ? p.sinks[h] : -INFINITY;
+    float m = sink;
+    for (int s = lane; s < p.nsplit; s += 64) m = fmaxf(m, p.mpart[s * rows + id]);
+    m = wave_max<64>(m);
+    const int c = lane % LG, g = lane / LG;
+    const float * src = p.opart + id * DV + blockIdx.y * CH + 4 * c;
+    wf4 o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int s0 = g; s0 < p.nsplit; s0 += 4 * GR) {
+        wf4 v[4];
+        float ms[4], ls[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i * GR;
+            const bool in = s < p.nsplit;
+            ms[i] = in ? p.mpart[s * rows + id] : -INFINITY;
+            ls[i] = in ? p.lpart[s * rows + id] : 0.f;
+            v[i] = ms[i] == -INFINITY && ls[i] == 0.f ? wf4{0.f, 0.f, 0.f, 0.f} : *(const wf4 *) (src + (size_t) s * rows * DV);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (!(ms[i] == -INFINITY && ls[i] == 0.f)) {        // a split that saw nothing left nothing to read
+                const float w = ms[i] == m ? 1.f : __builtin_amdgcn_exp2f((ms[i] - m) * FW_L2E);
+                l += ls[i] * w;
+                o += v[i] * w;
+            }
+    }
+    if constexpr (GR == 2) {
+        l += __shfl_xor(l, 32, 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 32, 64);
+    }
+    if (p.sinks) l += __builtin_amdgcn_exp2f((sink - m) * FW_L2E);
+    if (g) return;
+    const size_t t = id / p.H % p.n_q, seq = id / ((size_t) p.H * p.n_q);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *(wf4 *) (p.dst + (size_t) h * p.d1 + t * p.d2 + seq * p.d3 + 4 * (blockIdx.y * CH + 4 * c)) = o * inv;
+}
+
 // The mask's tile map: for 32 tokens x one key tile, whether some key is visible and whether some value
 // is not 0. Every head reads the same mask, so it is read once here instead of once a head; tiles
 // without a visible key are never loaded, tiles of zeros need no mask. One wave an entry.
@@ -945,27 +1038,39 @@ __global__ __launch_bounds__(256) void k_mask_map(const char * __restrict__ mask
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-struct FwPlan { bool wide, few; int rows, nsplit, n_tiles, n_tb; size_t part, map; };
+struct FwPlan { bool wide; int rows, nsplit, n_tiles, n_tb; size_t part, map; };
+constexpr size_t FW_JOIN_ROWS = 2048;   // from so many rows (times chunks) on the join takes a wave each: 4096 and four splits
+                                        // 35 against 40 us in all, 1024 and sixteen 30 against 27
 constexpr int FW_MAP_TOK = 17;   // from so many tokens on the tile map is built by a launch of its own
 
+// Rows of a workgroup and splits: those that end soonest by the times below, measured (us). A tile of a workgroup takes
+// t1 alone on its CU, t2 beside another (the absorbed form's tiles fill the LDS); its begin and end 6, the join 4 and
+// 1 for 8 MB of partial results. Absorbed, f16, 32 heads: 64 tokens, 1024 keys 35 with 32 rows and 4 splits (64 rows, 8
+// splits: 37); 512 tokens 285 with 64 rows (32: more than 400)
+// Expanded: 128 rows where they fill every CU twice (2048 tokens and keys, 32 heads: 118 against 134 with 64), else 64
+// (499 tokens: 26 against 39); 32 for no more rows than that (16 tokens, 1024 keys 14.6 against 15.8)
+struct FwRows { int rows; double t1, t2; };
 static FwPlan fw_plan(const ggml_tensor * dst) {
     const ggml_tensor * q = dst->src[0], * k = dst->src[1], * v = dst->src[2], * m = dst->src[3];
+    static const FwRows latent[2] = {{32, 1.33, 0}, {64, 1.63, 0}}, quant[1] = {{32, 1.8, 0}}, expanded[3] = {{32, 1.03, 1.27}, {64, 0.93, 1.46}, {128, 1.45, 2.8}};
     FwPlan p{};
     p.wide = k->ne[0] == 576;
     const int64_t G = q->ne[2] / k->ne[2], nrow = q->ne[1] * G, units = k->ne[2] * q->ne[3];
-    p.few = nrow <= 32;
-    p.rows = p.wide ? (p.few ? 32 : 64) : (p.few ? 32 : 128);
-    p.n_tiles = (int) mx_ceil_div(k->ne[1], FW_KT);
-    // splits: the number that ends soonest, counted in tile times on 256 CUs (one workgroup a CU: its
-    // tiles fill the LDS; two of the expanded form), against the join
-    const int64_t blocks = units * mx_ceil_div(nrow, p.rows), slots = p.wide ? 256 : 512;
-    int64_t best = INT64_MAX;
-    p.nsplit = 1;
-    for (int ns = 1; ns <= FW_MAX_SPLIT && ns <= p.n_tiles; ++ns) {
-        const int64_t cost = mx_ceil_div(blocks * ns, slots) * (mx_ceil_div(p.n_tiles, ns) * 2 + 1) + (ns > 1 ? 3 : 0);
-        if (cost < best) { best = cost; p.nsplit = ns; }
-    }
     const size_t rows = (size_t) q->ne[1] * q->ne[2] * q->ne[3];
+    p.n_tiles = (int) mx_ceil_div(k->ne[1], FW_KT);
+    const FwRows * cand = p.wide ? (k->type == GGML_TYPE_F16 ? latent : quant) : &expanded[nrow <= 32 ? 0 : units * mx_ceil_div(nrow, 128) >= 512 ? 2 : 1];
+    const int n_cand = p.wide && k->type == GGML_TYPE_F16 && nrow > 32 ? 2 : 1;
+    double best = 0;
+    for (int c = 0; c < n_cand; ++c) {
+        const int64_t blocks = units * mx_ceil_div(nrow, cand[c].rows);
+        for (int ns = 1; ns <= FW_MAX_SPLIT && ns <= p.n_tiles; ++ns) {
+            const int64_t n = blocks * ns, per = mx_ceil_div(p.n_tiles, ns);
+            const bool pair = !p.wide && n > 256;
+            const double us = (double) mx_ceil_div(n, pair ? 512 : 256) * ((double) per * (pair ? cand[c].t2 : cand[c].t1) + 6) +
+                              (ns > 1 ? 4 + (double) rows * ns * v->ne[0] * 1e-6 : 0);
+            if (p.nsplit == 0 || us < best) { best = us; p.nsplit = ns; p.rows = cand[c].rows; }
+        }
+    }
     p.part = p.nsplit > 1 ? (size_t) p.nsplit * rows : 0;
     p.n_tb = (int) mx_ceil_div(q->ne[1], FW_TB);
     if (m && m->ne[2] == 1 && q->ne[1] >= FW_MAP_TOK && p.n_tiles > 2) p.map = (size_t) m->ne[3] * p.n_tb * p.n_tiles;
@@ -1047,18 +1152,25 @@ void fa_wide_run(OpCtx & c, ggml_tensor * dst) {
     }
     MX_KLOG("fattn_wide DK=%d type=%d rows=%d nsplit=%d map=%d", (int) k->ne[0], (int) k->type, pl.rows, pl.nsplit, pl.map != 0);
     const dim3 grid((unsigned) (mx_ceil_div((int64_t) a.n_q * a.G, pl.rows) * a.Hkv * a.S), (unsigned) pl.nsplit);
-#define FL(T) do { if (pl.few) k_fattn_latent<T, 2><<<grid, 256, 0, c.st>>>(a); else k_fattn_latent<T, 4><<<grid, 512, 0, c.st>>>(a); } while (0)
     if (!pl.wide) {
-        if (pl.few) k_fattn_expanded<1, 2><<<grid, 128, 0, c.st>>>(a);
+        if (pl.rows == 32) k_fattn_expanded<1, 2><<<grid, 128, 0, c.st>>>(a);
+        else if (pl.rows == 64) k_fattn_expanded<1, 4><<<grid, 256, 0, c.st>>>(a);
         else        k_fattn_expanded<2, 4><<<grid, 256, 0, c.st>>>(a);
-    } else if (k->type == GGML_TYPE_F16) FL(GGML_TYPE_F16);
-    else if (k->type == GGML_TYPE_Q8_0) FL(GGML_TYPE_Q8_0);
-    else FL(GGML_TYPE_Q4_0);
-#undef FL
+    } else if (k->type == GGML_TYPE_Q8_0) k_fattn_latent<GGML_TYPE_Q8_0, 2><<<grid, FlGeo<GGML_TYPE_Q8_0, 2>::NT, 0, c.st>>>(a);
+    else if (k->type == GGML_TYPE_Q4_0) k_fattn_latent<GGML_TYPE_Q4_0, 2><<<grid, FlGeo<GGML_TYPE_Q4_0, 2>::NT, 0, c.st>>>(a);
+    else if (pl.rows == 32) k_fattn_latent<GGML_TYPE_F16, 2><<<grid, FlGeo<GGML_TYPE_F16, 2>::NT, 0, c.st>>>(a);
+    else k_fattn_latent<GGML_TYPE_F16, 4><<<grid, FlGeo<GGML_TYPE_F16, 4>::NT, 0, c.st>>>(a);
     if (pl.nsplit > 1) {
-        const dim3 grid((unsigned) (a.S * a.n_q * a.H), (unsigned) (DV / std::min(DV, 256)));
-        if (pl.wide) k_fattn_wide_join<512><<<grid, 256, 0, c.st>>>(a);
-        else         k_fattn_wide_join<128><<<grid, 256, 0, c.st>>>(a);
+        const unsigned rows = (unsigned) (a.S * a.n_q * a.H), chunks = (unsigned) (DV / std::min(DV, 256));
+        if (rows * (size_t) chunks >= FW_JOIN_ROWS) {
+            const dim3 grid((rows + 3) / 4, chunks);
+            if (pl.wide) k_fattn_wide_join_rows<512><<<grid, 256, 0, c.st>>>(a);
+            else         k_fattn_wide_join_rows<128><<<grid, 256, 0, c.st>>>(a);
+        } else {
+            const dim3 grid(rows, chunks);
+            if (pl.wide) k_fattn_wide_join<512><<<grid, 256, 0, c.st>>>(a);
+            else         k_fattn_wide_join<128><<<grid, 256, 0, c.st>>>(a);
+        }
     }
 }
 

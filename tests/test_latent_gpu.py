@@ -407,7 +407,7 @@ class Case:
 
 LATENT_SHAPES = [  # heads, n, m, S
     (4, 1, 1, 1), (16, 1, 63, 1), (32, 1, 64, 1), (32, 1, 65, 1), (10, 3, 300, 1), (32, 1, 1000, 3), (64, 1, 129, 2), (128, 1, 200, 1), (1, 1, 700, 1),
-    (40, 17, 150, 1), (8, 33, 200, 2), (4, 100, 100, 1), (16, 40, 640, 1), (1, 70, 70, 1),
+    (40, 17, 150, 1), (8, 33, 200, 2), (4, 100, 100, 1), (16, 40, 640, 1), (1, 70, 70, 1), (130, 64, 90, 1), (100, 10, 2000, 1),
 ]
 
 
@@ -420,7 +420,7 @@ def test_latent_attention(ctx, backend, cache, heads, n, m, S):
 
 
 @pytest.mark.parametrize("heads,kv_heads,n,m,S", [(4, 4, 1, 1, 1), (4, 4, 1, 333, 1), (4, 2, 20, 200, 1), (3, 3, 33, 64, 2), (8, 8, 5, 1200, 1), (8, 8, 130, 200, 1),
-                                                  (2, 2, 300, 517, 1), (16, 16, 64, 96, 1), (1, 1, 257, 257, 1), (6, 2, 50, 31, 1)])
+                                                  (2, 2, 300, 517, 1), (16, 16, 64, 96, 1), (1, 1, 257, 257, 1), (6, 2, 50, 31, 1), (520, 520, 65, 70, 1), (128, 64, 200, 230, 2)])
 def test_expanded_attention(ctx, backend, heads, kv_heads, n, m, S):
     mask = "causal" if m >= n else lambda rng, S, H, n, m: np.zeros((1, 1, n, m), np.float16)
     c = Case(ctx, form="expanded", heads=heads, kv_heads=kv_heads, n=n, m=m, S=S, mask=mask, seed=heads + n + m)
@@ -428,7 +428,8 @@ def test_expanded_attention(ctx, backend, heads, kv_heads, n, m, S):
 
 
 FORMS = [dict(form="latent", heads=8), dict(form="latent", heads=8, cache="q8_0"), dict(form="latent", heads=40), dict(form="latent", heads=40, cache="q4_0"),
-         dict(form="expanded", heads=4), dict(form="expanded", heads=4, n=150, m=170)]
+         dict(form="expanded", heads=4), dict(form="expanded", heads=4, n=150, m=170),
+         dict(form="latent", heads=128, n=70, m=110), dict(form="expanded", heads=512, n=66, m=80)]   # the variants of many rows
 
 
 def sized(form, n=3, m=170):
@@ -728,10 +729,11 @@ def test_graph_with_a_refused_node(pkg, ctx, backend):
 
 
 def test_kernel_choice(pkg, backend):
-    """few rows share the keys among the waves; more tokens than a few read the mask once for all heads"""
-    for kw, want in ((dict(heads=16, n=1, m=600), "rows=32"), (dict(heads=64, n=1, m=600), "rows=64"),
-                     (dict(heads=8, n=40, m=600), "map=1"), (dict(form="expanded", heads=2, n=100, m=600), "rows=128"),
-                     (dict(form="expanded", heads=2, n=1, m=600), "rows=32")):
+    """the rows of a workgroup go by the rows there are; more tokens than a few read the mask once for all heads"""
+    for kw, want in ((dict(heads=16, n=1, m=600), "rows=32 "), (dict(heads=130, n=64, m=90), "rows=64 nsplit=1 "), (dict(heads=100, n=10, m=2000), "rows=64 nsplit=16"),
+                     (dict(heads=130, n=64, m=90, cache="q4_0"), "rows=32 "), (dict(heads=8, n=40, m=600), "map=1"),
+                     (dict(form="expanded", heads=2, n=1, m=600), "rows=32 "), (dict(form="expanded", heads=2, n=100, m=600), "rows=64 "),
+                     (dict(form="expanded", heads=512, n=66, m=80), "rows=128 nsplit=1 ")):
         c = Case(pkg.Context(), **kw)
         backend.klog(True)
         c.run(backend)
