@@ -41,6 +41,7 @@ constexpr int FW_KT = 32;                    // keys of a tile
 constexpr int FW_PIECE = FW_KT * 128;        // 64 channels of a tile in LDS, f16
 constexpr int FW_TB = 32;                    // tokens of one entry of the mask's tile map
 constexpr int FW_MAX_SPLIT = 256;
+constexpr int FW_TILE = 0x3FFFFFFF;          // a listed tile's number; bit 30: the mask or the row's end cuts it
 constexpr float FW_L2E = 1.4426950408889634f;
 enum { FW_LIVE = 1, FW_MIXED = 2 };          // tile map bits: some key is visible; some mask value is not 0
 
@@ -130,6 +131,7 @@ __device__ __forceinline__ float fw_slope(const FwArgs & p, uint32_t h) {
 struct FwJob {
     int hk, seq, r0, nrow, split, nl;        // nl: tiles of the split
     const char * kb;
+    __device__ __forceinline__ int tile(const FwArgs & p, int i) const { return split + min(i, nl - 1) * p.nsplit; }   // the split's i-th (its last)
     __device__ __forceinline__ int head(const FwArgs & p, int r) const { return hk * p.G + r % p.G; }
     __device__ __forceinline__ const char * mask_row(const FwArgs & p, int tok, int h) const {
         return p.mask + (size_t) tok * p.m1 + (size_t) (h % p.mne2) * p.m2 + (size_t) (seq % p.mne3) * p.m3;
@@ -406,19 +408,26 @@ template <int KV, int RG> struct FlGeo {
 // the same barriers as the kernel below
 template <int KV, int ROWS>
 __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, char * const (&ring)[3], float (&dtop)[3][4]) {
-    // eight threads a row take two whole 32-blocks each, x and x + 8, and eight values of the last two blocks
-    constexpr int QB = qsize_of<KV>();
+    // eight threads a row take two whole 32-blocks each, x and x + 8, and eight values of the last two blocks. A block
+    // goes to LDS in four chunks of 8 values, thread x starting with the rot-th: the same chunk of all eight blocks
+    // would lie in the same banks (1160 of a tile's 2700 LDS cycles were conflicts)
+    constexpr int QB = qsize_of<KV>(), NL = KV == GGML_TYPE_Q8_0 ? 4 : 2;      // 8-byte loads of a block
     const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int row = tid >> 3, x8 = tid & 7, sw = fw_swz(row), pblk = 16 + (x8 >> 2), pval = 8 * (x8 & 3);
-    struct Regs { uint4 a[2], b[2]; uint2 w; uint16_t d[3]; } set[2];
+    const int row = tid >> 3, x8 = tid & 7, sw = fw_swz(row), pblk = 16 + (x8 >> 2), pval = 8 * (x8 & 3), rot = x8 >> 1;
+    int at[4], from[NL];                                        // places of the chunks, sources of the loads
+#pragma unroll
+    for (int c = 0; c < 4; ++c) at[c] = rot * FW_PIECE + 128 * row + 16 * ((4 * (x8 & 1) + ((c + rot) & 3)) ^ sw);
+#pragma unroll
+    for (int c = 0; c < NL; ++c) from[c] = x8 * QB + 2 + 8 * ((c + rot) & (NL - 1));
+    const int nib0 = rot & 2 ? 4 : 0, nib1 = (rot + 1) & 2 ? 4 : 0;            // 4 bits: shifts of chunks 0 and 1; 2 and 3 have the others
+    struct Regs { uint2 a[2][NL], w; uint16_t d[3]; } set[2];
     auto load = [&](int tile, Regs & q) __attribute__((always_inline)) {
-        const char * kr = j.kb + (size_t) min((tile & 0x3FFFFFFF) * FW_KT + row, p.n_kv - 1) * p.k1;
+        const char * kr = j.kb + (size_t) min((tile & FW_TILE) * FW_KT + row, p.n_kv - 1) * p.k1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const char * b = kr + (x8 + 8 * i) * QB;
-            q.d[i] = ld_u16(b);
-            q.a[i] = ldu16(b + 2);
-            if constexpr (KV == GGML_TYPE_Q8_0) q.b[i] = ldu16(b + 18);
+            q.d[i] = ld_u16(kr + (x8 + 8 * i) * QB);
+#pragma unroll
+            for (int c = 0; c < NL; ++c) __builtin_memcpy(&q.a[i][c], kr + from[c] + 8 * i * QB, 8);
         }
         const char * b = kr + pblk * QB;
         q.d[2] = ld_u16(b);
@@ -430,50 +439,38 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
         const uint32_t pr = __builtin_amdgcn_perm(0x64646464u, u, t ? 0x04030402u : 0x04010400u);
         return __builtin_bit_cast(uint32_t, __builtin_bit_cast(wh2, pr) - wh2{off, off});
     };
+    // a chunk: 8 values from 8 bytes, or from their nibbles at bit `sh`
+    auto chunk = [&](uint2 u, int sh) __attribute__((always_inline)) {
+        const uint32_t x = KV == GGML_TYPE_Q8_0 ? u.x ^ 0x80808080u : u.x >> sh & 0x0F0F0F0Fu, y = KV == GGML_TYPE_Q8_0 ? u.y ^ 0x80808080u : u.y >> sh & 0x0F0F0F0Fu;
+        return make_uint4(pair(x, 0), pair(x, 1), pair(y, 0), pair(y, 1));
+    };
     auto store = [&](const Regs & q, int slot) __attribute__((always_inline)) {
         char * const buf = ring[slot];
         uint16_t * const steps = (uint16_t *) (buf + 9 * FW_PIECE);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int b = x8 + 8 * i;
-            uint32_t w[16];                                     // 32 values in order, as f16 pairs
-            if constexpr (KV == GGML_TYPE_Q8_0) {
-                const uint32_t src[8] = {q.a[i].x, q.a[i].y, q.a[i].z, q.a[i].w, q.b[i].x, q.b[i].y, q.b[i].z, q.b[i].w};
-#pragma unroll
-                for (int c = 0; c < 16; ++c) w[c] = pair(src[c >> 1] ^ 0x80808080u, c & 1);
-            } else {
-                const uint32_t src[4] = {q.a[i].x, q.a[i].y, q.a[i].z, q.a[i].w};
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {                   // low nibbles are values 0..15, high 16..31
-                    w[c] = pair(src[c >> 1] & 0x0F0F0F0Fu, c & 1);
-                    w[c + 8] = pair(src[c >> 1] >> 4 & 0x0F0F0F0Fu, c & 1);
-                }
-            }
-            steps[b * FW_KT + row] = q.d[i];
-            char * kd = buf + (b >> 1) * FW_PIECE + 128 * row;
+            steps[(x8 + 8 * i) * FW_KT + row] = q.d[i];
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                *(uint4 *) (kd + 16 * ((4 * (b & 1) + c) ^ sw)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const uint32_t u = c < 2 ? q.w.x : q.w.y;
-            w[c] = pair(KV == GGML_TYPE_Q8_0 ? u ^ 0x80808080u : (pval & 16 ? u >> 4 : u) & 0x0F0F0F0Fu, c & 1);
+                *(uint4 *) (buf + at[c] + 4 * i * FW_PIECE) = chunk(q.a[i][c & (NL - 1)], c == 0 ? nib0 : c == 1 ? nib1 : c == 2 ? 4 - nib0 : 4 - nib1);
         }
         steps[pblk * FW_KT + row] = q.d[2];
-        *(uint4 *) (buf + 8 * FW_PIECE + 128 * row + 16 * ((x8 & 7) ^ sw)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *(uint4 *) (buf + 8 * FW_PIECE + 128 * row + 16 * (x8 ^ sw)) = chunk(q.w, pval & 16 ? 4 : 0);
         const float top = wave_max<64>(fmaxf(fmaxf(fabsf(h2f(q.d[0])), fabsf(h2f(q.d[1]))), fabsf(h2f(q.d[2]))));
         if (lane == 0) dtop[slot][wave] = top;
     };
 
+    // the split's first two tiles on their way while the tiles are listed; as a rule they are the list's
+    const int s0 = j.tile(p, 0), s1 = j.tile(p, 1);
+    load(s0, set[0]);
+    if (j.nl > 1) load(s1, set[1]);
     FwTiles tiles;
     tiles.w0 = 0;
     tiles.window<ROWS>(p, j);
     // the first two tiles stored, the third and fourth in registers
     int t0 = tiles.next<ROWS>(p, j), t1 = t0 >= 0 ? tiles.next<ROWS>(p, j) : -1;
-    if (t0 >= 0) load(t0, set[0]);
-    if (t1 >= 0) load(t1, set[1]);
+    if (t0 >= 0 && (t0 & FW_TILE) != s0) load(t0, set[0]);
+    if (t1 >= 0 && (t1 & FW_TILE) != s1) load(t1, set[1]);
     int t2 = t1 >= 0 ? tiles.next<ROWS>(p, j) : -1, t3 = t2 >= 0 ? tiles.next<ROWS>(p, j) : -1;
     if (t0 >= 0) store(set[0], 0);
     if (t2 >= 0) load(t2, set[0]);
@@ -525,32 +522,44 @@ __global__ __launch_bounds__((FlGeo<KV, RG>::NT), (FlGeo<KV, RG>::NT / 256)) voi
     }
     float qx[NS][8];
     fw_query<NS>(p, j, r, NS * dh, qx);                         // (on its way while the tiles are listed)
-    FwTiles tiles;
-    tiles.w0 = 0;
-    tiles.window<ROWS>(p, j);
-
     // ---- staging. f16: instruction x of a tile fills rows 8 (x & 3) .. + 7 of piece x >> 2; lane l brings
     // the chunk that belongs at its place, (l % 8) ^ swz(row) of row l / 8
     const int srow = 8 * (wave & 3) + (lane >> 3), ssrc = 16 * ((lane & 7) ^ fw_swz(srow));
-    auto dma_off = [&](int tile) { return min(srow, p.n_kv - 1 - (tile & 0x3FFFFFFF) * FW_KT) * (int) p.k1 + ssrc; };
-    auto dma_src = [&](int tile) { return fw_src(j.kb + (size_t) ((tile & 0x3FFFFFFF) * FW_KT) * p.k1); };
+    auto dma_off = [&](int tile) { return min(srow, p.n_kv - 1 - (tile & FW_TILE) * FW_KT) * (int) p.k1 + ssrc; };
+    auto dma_src = [&](int tile) { return fw_src(j.kb + (size_t) ((tile & FW_TILE) * FW_KT) * p.k1); };
     // instruction i of a wave: it keeps to one row group (wave & 3); of eight waves, two share one and halve its pieces
     auto dma = [&](const FwSrc & src, int off, char * buf, int i) __attribute__((always_inline)) {
         const int piece = NW == 8 ? min(2 * i + (wave >> 2), 8) : i;        // (piece 8 is brought twice)
         fw_dma(src, off, 128 * piece, buf + piece * FW_PIECE + 1024 * (wave & 3));
     };
-    // ---- the first tiles on their way, then the query rows. id[c]: the tile in slot c of the ring (-1: none)
+    // ---- the split's first tiles on their way while the tiles are listed; as a rule they are the list's.
+    // id[c]: the tile in slot c of the ring (-1: none)
     char * const ring[4] = {t0, t1, t2, t3};
     int id[RING];
+    auto dma_tile = [&](int tile, char * buf) __attribute__((always_inline)) {
+        const FwSrc src = dma_src(tile);
+        const int off = dma_off(tile);
+#pragma unroll
+        for (int i = 0; i < geo::DMA; ++i) dma(src, off, buf, i);
+    };
+    if constexpr (!QUANT) {
+#pragma unroll
+        for (int c = 0; c < RING - 1; ++c) if (c < j.nl) dma_tile(j.tile(p, c), ring[c]);
+    }
+    FwTiles tiles;
+    tiles.w0 = 0;
+    tiles.window<ROWS>(p, j);
+    bool listed = true;
 #pragma unroll
     for (int c = 0; c < RING - 1; ++c) {
         id[c] = c == 0 || id[c - 1] >= 0 ? tiles.next<ROWS>(p, j) : -1;
-        if constexpr (!QUANT) {
-            if (id[c] < 0) continue;
-            const FwSrc src = dma_src(id[c]);
-            const int off = dma_off(id[c]);
+        listed &= id[c] < 0 || (id[c] & FW_TILE) == j.tile(p, c);
+    }
+    if constexpr (!QUANT) {
+        if (!listed) {
+            fw_vmcnt<0>();                                      // (behind the ones under way to the same places)
 #pragma unroll
-            for (int i = 0; i < geo::DMA; ++i) dma(src, off, ring[c], i);
+            for (int c = 0; c < RING - 1; ++c) if (id[c] >= 0) dma_tile(id[c], ring[c]);
         }
     }
     id[RING - 1] = id[RING - 2] >= 0 ? tiles.next<ROWS>(p, j) : -1;         // fetched by the first body
@@ -678,7 +687,7 @@ __global__ __launch_bounds__((FlGeo<KV, RG>::NT), (FlGeo<KV, RG>::NT / 256)) voi
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = p.softcap * tanhf(s[i >> 2][i & 3]);
         }
-        if (tile >> 30) fw_mask(p, j, r, tile & 0x3FFFFFFF, s);
+        if (tile >> 30) fw_mask(p, j, r, tile & FW_TILE, s);
         if constexpr (QUANT) {
             float top = 0.f;
 #pragma unroll
@@ -791,7 +800,7 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     tiles.window<ROWS>(p, j);
     const int srow = lane >> 3, ssrc = 16 * ((lane & 7) ^ fw_swz(8 * wave + srow));   // (W is even: the same for rb below)
     auto dma = [&](int tile, char * buf) {
-        const int key0 = (tile & 0x3FFFFFFF) * FW_KT;
+        const int key0 = (tile & FW_TILE) * FW_KT;
         const FwSrc ks = fw_src(j.kb + (size_t) key0 * p.k1), vs = fw_src(vb + (size_t) key0 * p.v1);
 #pragma unroll
         for (int b = 0; b < 4 / W; ++b) {
@@ -867,7 +876,7 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
         }
         if (id[C] >> 30) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) fw_mask(p, j, min(rg0 + 16 * nt + n16, j.nrow - 1), id[C] & 0x3FFFFFFF, s[nt]);
+            for (int nt = 0; nt < NT; ++nt) fw_mask(p, j, min(rg0 + 16 * nt + n16, j.nrow - 1), id[C] & FW_TILE, s[nt]);
         }
         wh4 v[3][2];
         auto ldv = [&](int d) {
@@ -920,33 +929,35 @@ __global__ __launch_bounds__(256) void k_fattn_wide_join(FwArgs p) {
     __shared__ float wgt[FW_MAX_SPLIT];
     __shared__ float red[16];
     __shared__ __align__(16) wf4 part[GR][LG];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, c = tid % LG, g = tid / LG;
     const size_t rows = (size_t) p.S * p.n_q * p.H, id = blockIdx.x;
     const int h = (int) (id % p.H);
+    const float * src = p.opart + id * DV + blockIdx.y * CH + 4 * c;
+    wf4 v[8];
+    auto fetch = [&](int s0) __attribute__((always_inline)) {   // (a split that saw nothing left nothing: read and not used)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = *(const wf4 *) (src + (size_t) min(s0 + i * GR, p.nsplit - 1) * rows * DV);
+    };
+    fetch(g);                                                   // on their way while the weights are computed
     float ms = -INFINITY, ls = 0.f;                             // a thread a split
     if (tid < p.nsplit) { ms = p.mpart[tid * rows + id]; ls = p.lpart[tid * rows + id]; }
     float m = block_max(ms, red);
     if (p.sinks) m = fmaxf(m, p.sinks[h]);
-    const bool none = ms == -INFINITY && ls == 0.f;             // a split that saw nothing left nothing to read
+    const bool none = ms == -INFINITY && ls == 0.f;
     const float w = none ? 0.f : ms == m ? 1.f : __builtin_amdgcn_exp2f((ms - m) * FW_L2E);
     wgt[tid] = none ? -1.f : w;
     float l = block_sum(ls * w, red);
     if (p.sinks) l += __builtin_amdgcn_exp2f((p.sinks[h] - m) * FW_L2E);
     __syncthreads();
-    const int c = tid % LG, g = tid / LG;
-    const float * src = p.opart + id * DV + blockIdx.y * CH + 4 * c;
     wf4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = g; s0 < p.nsplit; s0 += 8 * GR) {
-        wf4 v[8];
-        float a[8];
+        if (s0 != g) fetch(s0);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int s = s0 + i * GR;
-            a[i] = s < p.nsplit ? wgt[s] : -1.f;
-            v[i] = a[i] < 0.f ? wf4{0.f, 0.f, 0.f, 0.f} : *(const wf4 *) (src + (size_t) s * rows * DV);
+            const float a = s < p.nsplit ? wgt[s] : -1.f;
+            if (!(a < 0.f)) o += v[i] * a;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) if (!(a[i] < 0.f)) o += v[i] * a[i];
     }
     part[g][c] = o;
     __syncthreads();
