@@ -117,7 +117,7 @@ bool rope_axes_supported(const ggml_tensor * dst) {
         }
         default: return false;
     }
-    if (rope_pairs(mode, n_dims) > MX_ROPE_MAXP || x->ne[1] > INT32_MAX || x->ne[2] * x->ne[3] > INT32_MAX) return false;
+    if (rope_pairs(mode, n_dims) > MX_ROPE_MAXP || x->ne[0] * x->ne[1] > INT32_MAX / 2 || x->ne[2] * x->ne[3] > INT32_MAX) return false;
     return rope_pos_ok(dst);
 }
 
@@ -366,7 +366,8 @@ static bool row_dst(const ggml_tensor * sr, int64_t n, RowDst * d) {
 // RMS_NORM -> MUL, ROPE -> CONCAT -> SET_ROWS (the pair and ROPE in either order, CONCAT either way
 // round); views between them. Nothing else may read the members' results, except the MUL's, which is
 // written as well then. Positions enter by the same functions as the unfused ROPE, so fusing changes
-// no angle.
+// no angle. Tokens of one cell are written by workgroups that know nothing of each other, as by SET_ROWS: the cell
+// holds values of any of them.
 int fuse_append_rows(OpCtx & c, ggml_cgraph * g, int i, const UseCount & use_map) {
     static const bool off = getenv("GGML_MI355X_NO_APPEND_FUSION") != nullptr;   // A/B
     if (off) return 0;

@@ -392,22 +392,236 @@ __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, cons
 // much for one wave beside the rest of it, so the pair shares: wave dh multiplies channels [288 dh, + 288)
 // of the keys, the halves of the scores are exchanged through LDS (the only barrier of a tile), both do
 // the softmax, and each keeps half of the output channels.
-// A quantised cache takes four waves more, one a SIMD, that turn the blocks into f16 integers ahead of the others:
-// done by the same waves it left the matrix unit idle (4 bits 2.6 us a tile instead of 1.8).
-template <int KV, int RG> struct FlGeo {
-    static constexpr bool QUANT = KV != GGML_TYPE_F16;
-    static constexpr int NT = 128 * RG + (QUANT ? 256 : 0);     // threads
+template <int RG> struct FlGeo {
+    static constexpr int NT = 128 * RG;                         // threads
     // tiles in the ring, three ahead of the one in use where they fit beside the exchange
-    static constexpr int RING = !QUANT && RG == 2 ? 4 : 3;
-    static constexpr int STEPS = QUANT ? 18 * FW_KT * 2 : 0;    // the blocks' steps, [block][key] f16
-    static constexpr int BUF = 9 * FW_PIECE + STEPS;
+    static constexpr int RING = RG == 2 ? 4 : 3;
+    static constexpr int BUF = 9 * FW_PIECE;
     static constexpr int DMA = (36 + 2 * RG - 1) / (2 * RG);    // LDS-DMA instructions of a wave and tile
 };
 
-// The producers of a quantised cache: blocks through registers, two tiles ahead of the store, into the slots of the ring;
-// the same barriers as the kernel below
+template <int RG>
+__global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
+    using geo = FlGeo<RG>;
+    constexpr int RING = geo::RING, NS = 9, ND = 16, ROWS = 16 * RG, NW = 2 * RG;
+    // the ring's tiles as objects of their own: reads of one need not wait for the DMA that fills another
+    __shared__ __align__(128) char t0[geo::BUF];
+    __shared__ __align__(128) char t1[geo::BUF];
+    __shared__ __align__(128) char t2[geo::BUF];
+    __shared__ __align__(128) char t3[RING == 4 ? geo::BUF : 16];
+    __shared__ __align__(16) wf4 exch[2][NW][2][64];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n16 = lane & 15, g4 = lane >> 4;
+    const int rg = wave >> 1, dh = wave & 1;
+    const FwJob j = fw_job<ROWS, false>(p);
+    const int r = min(j.r0 + 16 * rg + n16, j.nrow - 1);        // this lane's row
+
+    float qx[NS][8];
+    fw_query<NS>(p, j, r, NS * dh, qx);                         // (on its way while the tiles are listed)
+    // ---- staging: instruction x of a tile fills rows 8 (x & 3) .. + 7 of piece x >> 2; lane l brings
+    // the chunk that belongs at its place, (l % 8) ^ swz(row) of row l / 8
+    const int srow = 8 * (wave & 3) + (lane >> 3), ssrc = 16 * ((lane & 7) ^ fw_swz(srow));
+    auto dma_off = [&](int tile) { return min(srow, p.n_kv - 1 - (tile & FW_TILE) * FW_KT) * (int) p.k1 + ssrc; };
+    auto dma_src = [&](int tile) { return fw_src(j.kb + (size_t) ((tile & FW_TILE) * FW_KT) * p.k1); };
+    // instruction i of a wave: it keeps to one row group (wave & 3); of eight waves, two share one and halve its pieces
+    auto dma = [&](const FwSrc & src, int off, char * buf, int i) __attribute__((always_inline)) {
+        const int piece = NW == 8 ? min(2 * i + (wave >> 2), 8) : i;        // (piece 8 is brought twice)
+        fw_dma(src, off, 128 * piece, buf + piece * FW_PIECE + 1024 * (wave & 3));
+    };
+    // ---- the split's first tiles on their way while the tiles are listed; as a rule they are the list's.
+    // id[c]: the tile in slot c of the ring (-1: none)
+    char * const ring[4] = {t0, t1, t2, t3};
+    int id[RING];
+    auto dma_tile = [&](int tile, char * buf) __attribute__((always_inline)) {
+        const FwSrc src = dma_src(tile);
+        const int off = dma_off(tile);
+#pragma unroll
+        for (int i = 0; i < geo::DMA; ++i) dma(src, off, buf, i);
+    };
+#pragma unroll
+    for (int c = 0; c < RING - 1; ++c) if (c < j.nl) dma_tile(j.tile(p, c), ring[c]);
+    FwTiles tiles;
+    tiles.w0 = 0;
+    tiles.window<ROWS>(p, j);
+    bool listed = true;
+#pragma unroll
+    for (int c = 0; c < RING - 1; ++c) {
+        id[c] = c == 0 || id[c - 1] >= 0 ? tiles.next<ROWS>(p, j) : -1;
+        listed &= id[c] < 0 || (id[c] & FW_TILE) == j.tile(p, c);
+    }
+    if (!listed) {
+        fw_vmcnt<0>();                                          // (behind the ones under way to the same places)
+#pragma unroll
+        for (int c = 0; c < RING - 1; ++c) if (id[c] >= 0) dma_tile(id[c], ring[c]);
+    }
+    id[RING - 1] = id[RING - 2] >= 0 ? tiles.next<ROWS>(p, j) : -1;         // fetched by the first body
+    wh8 qh[NS], ql[NS];
+    const float qsc = fw_terms<NS>(p, qx, qh, ql);              // of this half's part of the scores
+
+    wf4 o[ND];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = wf4{0.f, 0.f, 0.f, 0.f};
+    // per-lane LDS offsets: step i of this wave's half is step gs = 9 dh + i of the row, chunk g4 of half gs & 1 of piece gs >> 1
+    const int kx0 = 128 * n16 + 16 * (g4 ^ fw_swz(n16)), kx1 = 128 * n16 + 16 * ((4 + g4) ^ fw_swz(n16));
+    const int ka0 = dh ? kx1 + 4 * FW_PIECE : kx0, ka1 = dh ? kx0 + 5 * FW_PIECE : kx1;
+    const int iq = (lane >> 2) & 3, ip = lane & 3, vrow = 4 * g4 + iq, vsw = fw_swz(vrow);
+    int va[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) va[i] = (4 * dh + p.vpiece) * FW_PIECE + 128 * vrow + 16 * ((2 * i + (ip >> 1)) ^ vsw) + 8 * (ip & 1);
+
+    int par = 0;
+    wf4 s[2], t[2];                                             // the scores of the tile in hand, this half's of the next
+    float ms = 0.f;
+    wh8 ph, pl;
+    float e[8];
+    // fragments from LDS are read AK (AV) steps ahead: with eight waves at it a read takes some 250 cycles, a step's
+    // matrix instructions 64. The first ones before the barrier's other business, and before the end of the scores
+    constexpr int AK = 4, AV = 3;
+    wh8 a[AK + 1][2], v[AV + 1][2];
+    auto lda = [&](const char * buf, int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) a[i % (AK + 1)][u] = *(const wh8 *) (buf + (i & 1 ? ka1 : ka0) + (i >> 1) * FW_PIECE + 2048 * u);
+    };
+    auto ldv = [&](const char * buf, int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const char * a_ = buf + va[2 * (b & 1) + c] + (b >> 1) * FW_PIECE;
+            const wh4 v0 = lds_tr4(a_), v1 = lds_tr4(a_ + 2048);
+            v[b % (AV + 1)][c] = wh8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        }
+    };
+    auto ahead = [&](const char * buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < AK; ++i) lda(buf, i);
+    };
+    // this half's part of the scores of the tile in `buf` to the exchange; meanwhile (W) the weights of the tile in
+    // hand, whose values lie in `vbuf`
+    // and a further tile goes to `fbuf`: instruction by instruction here, where the matrix unit hides them (all at once
+    // behind the barrier they took 800 cycles). They run on past the last tile, into places no longer read
+    auto scores = [&](const char * buf, const char * vbuf, char * fbuf, const FwSrc & fsrc, int foff, auto with) __attribute__((always_inline)) {
+        constexpr bool W = decltype(with)::value;
+        t[0] = t[1] = wf4{0.f, 0.f, 0.f, 0.f};
+        wf4 tl[2] = {t[0], t[0]};                               // a chain of its own for the low term
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            if constexpr (W) { if (i < geo::DMA) dma(fsrc, foff, fbuf, i); }
+            if (i + AK < NS) lda(buf, i + AK);
+            if (W && i >= NS - AV) ldv(vbuf, i - (NS - AV));
+#pragma unroll
+            for (int u = 0; u < 2; ++u) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], t[u], 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) tl[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], tl[u], 0, 0, 0);
+            if constexpr (W) {
+                if (i < 8) {
+                    e[i] = fw_weight(s, i, ms);
+                    l += e[i];
+                    if (i & 1) split2(e[i - 1], e[i], i - 1, ph, pl);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        t[0] = (t[0] + tl[0]) * qsc;
+        t[1] = (t[1] + tl[1]) * qsc;
+        exch[par][wave][0][lane] = t[0];
+        exch[par][wave][1][lane] = t[1];
+    };
+    // behind the barrier: the scores of tile `tile` (slot C) whole, the reference maximum; the first fragments of the
+    // tile in `buf` meanwhile
+    auto whole = [&](int tile, const int C, const char * buf) __attribute__((always_inline)) {
+        const wf4 x0 = exch[par][wave ^ 1][0][lane], x1 = exch[par][wave ^ 1][1][lane];
+        __builtin_amdgcn_sched_barrier(0);
+        ahead(buf);
+        s[0] = t[0] + x0;
+        s[1] = t[1] + x1;
+        par ^= 1;
+        if (p.softcap != 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = p.softcap * tanhf(s[i >> 2][i & 3]);
+        }
+        if (tile >> 30) fw_mask(p, j, r, tile & FW_TILE, s);
+        ms = fw_raise<ND>(s, m, l, o);
+    };
+    // O^T += V^T P^T: keys 4 g4 + 0..3 of the two 16-key blocks a lane, as the scores lie; 32 channels at a
+    // time, so that a term's product does not wait for the other's
+    auto values = [&](const char * buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < ND / 2; ++b) {
+            if (b + AV < ND / 2) ldv(buf, b + AV);
+            o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], ph, o[2 * b], 0, 0, 0);
+            o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], ph, o[2 * b + 1], 0, 0, 0);
+            o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], pl, o[2 * b], 0, 0, 0);
+            o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], pl, o[2 * b + 1], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // the tile in slot C, its scores in hand, with the next tile's scores on the way: the weights are taken among the
+    // matrix instructions of the next tile's scores, the exchange passes under this tile's values. The barrier then
+    // frees slot C (and tells that the tile after the next is whole)
+    auto body = [&](auto slot_) __attribute__((always_inline)) {
+        constexpr int C = decltype(slot_)::value, C1 = (C + 1) % RING, F = (C + RING - 1) % RING;
+        const int further = id[F] >= 0 ? id[F] : id[C];         // (behind the last tile: any, into a place no longer read)
+        scores(ring[C1], ring[C], ring[F], dma_src(further), dma_off(further), std::true_type{});
+        values(ring[C]);
+        fw_vmcnt<(RING - 3) * geo::DMA>();                      // the tile after the next has landed
+        fw_barrier();
+        id[C] = id[F] >= 0 ? tiles.next<ROWS>(p, j) : -1;
+        whole(id[C1], C1, ring[(C + 2) % RING]);                // (fragments read for nothing where no such tile is left)
+    };
+
+    fw_vmcnt<0>();
+    __syncthreads();
+    if (id[0] >= 0) {
+        ahead(t0);
+        scores(t0, t0, nullptr, dma_src(id[0]), 0, std::false_type{});
+        fw_barrier();
+        whole(id[0], 0, t1);
+        const char * last;
+        for (;;) {
+            last = t0;
+            if (id[1] < 0) break;
+            body(std::integral_constant<int, 0>{});
+            last = t1;
+            if (id[2] < 0) break;
+            body(std::integral_constant<int, 1>{});
+            last = t2;
+            if (id[3 % RING] < 0) break;
+            body(std::integral_constant<int, 2>{});
+            if constexpr (RING == 4) {
+                last = t3;
+                if (id[0] < 0) break;
+                body(std::integral_constant<int, 3>{});
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            e[i] = fw_weight(s, i, ms);
+            l += e[i];
+            if (i & 1) split2(e[i - 1], e[i], i - 1, ph, pl);
+        }
+        fw_vmcnt<0>();                                          // no DMA outlives the workgroup's LDS
+#pragma unroll
+        for (int b = 0; b < AV; ++b) ldv(last, b);
+        values(last);
+    }
+    fw_store<576, 512, GGML_TYPE_F16, ND>(p, j, j.kb, p.k1, 64 * p.vpiece, j.r0 + 16 * rg, 256 * dh, m, l, o);
+}
+
+// ---- absorbed, quantised ------------------------------------------------------------------------------
+// 32 rows, and the work of a tile dealt out by kind, one wave of each kind a SIMD, so that one's waits are filled by the
+// others' vector instructions (they bound it: a block's step enters its products, and V's steps the weights, in 32 bits):
+//   4 waves   scores of the next tile (a pair of waves a row group, as above), its softmax; the weights go through LDS
+//   4 waves   values of this tile, half of the channels of a row group each
+//   4 waves   blocks of the tile after the next into f16 integers
+// Two barriers a tile: behind the halves of the scores, and behind the weights. A tile on every CU at once, 4 bits: 2.6 us
+// with all of it in one wave a SIMD, 2.2 with the last kind apart, 2.1 so; alone on the chip 2.6, 1.8 and 1.7. What is left
+// is the vector unit's: 600 instructions a SIMD and tile, 5 cycles each (the matrix unit's 68 take 1100 cycles beside them)
+constexpr int FQ_BUF = 9 * FW_PIECE + 18 * FW_KT * 2;           // a tile and its blocks' steps, [block][key] f16
+
+// the last kind: blocks through registers, two tiles ahead of the store
 template <int KV, int ROWS>
-__device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, char * const (&ring)[3], float (&dtop)[3][4]) {
+__device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, char * ring, float (&dtop)[3][4]) {
     // eight threads a row take two whole 32-blocks each, x and x + 8, and eight values of the last two blocks. A block
     // goes to LDS in four chunks of 8 values, thread x starting with the rot-th: the same chunk of all eight blocks
     // would lie in the same banks (1160 of a tile's 2700 LDS cycles were conflicts)
@@ -444,16 +658,14 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
         const uint32_t x = KV == GGML_TYPE_Q8_0 ? u.x ^ 0x80808080u : u.x >> sh & 0x0F0F0F0Fu, y = KV == GGML_TYPE_Q8_0 ? u.y ^ 0x80808080u : u.y >> sh & 0x0F0F0F0Fu;
         return make_uint4(pair(x, 0), pair(x, 1), pair(y, 0), pair(y, 1));
     };
-    auto store = [&](const Regs & q, int slot) __attribute__((always_inline)) {
-        char * const buf = ring[slot];
+    auto store = [&](const Regs & q, int slot, int half) __attribute__((always_inline)) {
+        char * const buf = ring + slot * FQ_BUF;
         uint16_t * const steps = (uint16_t *) (buf + 9 * FW_PIECE);
+        steps[(x8 + 8 * half) * FW_KT + row] = q.d[half];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            steps[(x8 + 8 * i) * FW_KT + row] = q.d[i];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                *(uint4 *) (buf + at[c] + 4 * i * FW_PIECE) = chunk(q.a[i][c & (NL - 1)], c == 0 ? nib0 : c == 1 ? nib1 : c == 2 ? 4 - nib0 : 4 - nib1);
-        }
+        for (int c = 0; c < 4; ++c)
+            *(uint4 *) (buf + at[c] + 4 * half * FW_PIECE) = chunk(q.a[half][c & (NL - 1)], c == 0 ? nib0 : c == 1 ? nib1 : c == 2 ? 4 - nib0 : 4 - nib1);
+        if (half == 0) return;
         steps[pblk * FW_KT + row] = q.d[2];
         *(uint4 *) (buf + 8 * FW_PIECE + 128 * row + 16 * (x8 ^ sw)) = chunk(q.w, pval & 16 ? 4 : 0);
         const float top = wave_max<64>(fmaxf(fmaxf(fabsf(h2f(q.d[0])), fabsf(h2f(q.d[1]))), fabsf(h2f(q.d[2]))));
@@ -467,152 +679,181 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
     FwTiles tiles;
     tiles.w0 = 0;
     tiles.window<ROWS>(p, j);
-    // the first two tiles stored, the third and fourth in registers
-    int t0 = tiles.next<ROWS>(p, j), t1 = t0 >= 0 ? tiles.next<ROWS>(p, j) : -1;
-    if (t0 >= 0 && (t0 & FW_TILE) != s0) load(t0, set[0]);
-    if (t1 >= 0 && (t1 & FW_TILE) != s1) load(t1, set[1]);
-    int t2 = t1 >= 0 ? tiles.next<ROWS>(p, j) : -1, t3 = t2 >= 0 ? tiles.next<ROWS>(p, j) : -1;
-    if (t0 >= 0) store(set[0], 0);
-    if (t2 >= 0) load(t2, set[0]);
-    if (t1 >= 0) store(set[1], 1);
-    if (t3 >= 0) load(t3, set[1]);
+    // tile 0 stored, 1 and 2 in registers
+    int t0 = tiles.next<ROWS>(p, j), t1 = t0 >= 0 ? tiles.next<ROWS>(p, j) : -1, t2 = t1 >= 0 ? tiles.next<ROWS>(p, j) : -1;
+    if (t0 >= 0) {
+        if ((t0 & FW_TILE) != s0) load(t0, set[0]);
+        if (t1 >= 0 && (t1 & FW_TILE) != s1) load(t1, set[1]);
+        store(set[0], 0, 0);
+        store(set[0], 0, 1);
+        if (t2 >= 0) load(t2, set[0]);
+    }
     fw_barrier();
-    if (t0 < 0) return;
-    fw_barrier();
-    // beside tile i + 1's scores and tile i's values: tile i + 2 to its slot, tile i + 4 on its way
-    auto body = [&](auto i_) __attribute__((always_inline)) {
-        constexpr int I = decltype(i_)::value;
-        if (t1 < 0) return false;
-        if (t2 >= 0) store(set[I & 1], (I + 2) % 3);
-        const int t4 = t3 >= 0 ? tiles.next<ROWS>(p, j) : -1;
-        if (t4 >= 0) load(t4, set[I & 1]);
-        t1 = t2; t2 = t3; t3 = t4;
+    // beside tile i's scores: tile i + 1 to its slot, tile i + 3 on its way
+    int slot = 1;
+    auto body = [&](Regs & q) __attribute__((always_inline)) {
+        if (t0 < 0) return false;
+        if (t1 >= 0) store(q, slot, 0);
+        fw_barrier();
+        if (t1 >= 0) store(q, slot, 1);
+        const int t3 = t2 >= 0 ? tiles.next<ROWS>(p, j) : -1;
+        if (t3 >= 0) load(t3, q);
+        t0 = t1; t1 = t2; t2 = t3;
+        slot = slot == 2 ? 0 : slot + 1;
         fw_barrier();
         return true;
     };
-    while (body(std::integral_constant<int, 0>{}) && body(std::integral_constant<int, 1>{}) && body(std::integral_constant<int, 2>{}) &&
-           body(std::integral_constant<int, 3>{}) && body(std::integral_constant<int, 4>{}) && body(std::integral_constant<int, 5>{})) {}
+    while (body(set[1]) && body(set[0])) {}
+    fw_barrier();
 }
 
-template <int KV, int RG>
-__global__ __launch_bounds__((FlGeo<KV, RG>::NT), (FlGeo<KV, RG>::NT / 256)) void k_fattn_latent(FwArgs p) {
-    using geo = FlGeo<KV, RG>;
-    constexpr bool QUANT = geo::QUANT;
-    constexpr int RING = geo::RING, NS = 9, ND = 16, ROWS = 16 * RG, NW = 2 * RG;
-    // the ring's tiles as objects of their own: reads of one need not wait for the DMA that fills another
-    __shared__ __align__(128) char t0[geo::BUF];
-    __shared__ __align__(128) char t1[geo::BUF];
-    __shared__ __align__(128) char t2[geo::BUF];
-    __shared__ __align__(128) char t3[RING == 4 ? geo::BUF : 16];
-    __shared__ __align__(16) wf4 exch[2][NW][2][64];
-    __shared__ __align__(16) float dtop[QUANT ? 3 : 1][4];      // the tiles' largest steps, wave by wave
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n16 = lane & 15, g4 = lane >> 4;
-    const int rg = wave >> 1, dh = wave & 1;
+template <int KV>
+__global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
+    constexpr int NS = 9, ND = 16, ROWS = 32, AK = 2, AV = 2;   // fragments from LDS are read AK (AV) steps ahead
+    __shared__ __align__(128) char ring[3 * FQ_BUF];
+    __shared__ __align__(16) wf4 exch[4][2][64];                // halves of scores
+    __shared__ __align__(16) wf4 wgt[2][2][64];                 // weights: row group, 16 keys, the scores' lane
+    __shared__ float scl[2][16];                                // a row's O takes this factor before them
+    __shared__ __align__(16) float dtop[3][4];                  // the tiles' largest steps, wave by wave
+    __shared__ float endm[2][64], endl[2][2][64];
+    __shared__ int endq;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n16 = lane & 15, g4 = lane >> 4, rg = wave >> 1 & 1, dh = wave & 1;
     const FwJob j = fw_job<ROWS, false>(p);
+    if (wave >= 8) {
+        fw_produce<KV, ROWS>(p, j, ring, dtop);
+        return;
+    }
     const int r = min(j.r0 + 16 * rg + n16, j.nrow - 1);        // this lane's row
-
-    if constexpr (QUANT) {
-        if (wave >= NW) {
-            char * const ring[3] = {t0, t1, t2};
-            fw_produce<KV, ROWS>(p, j, ring, dtop);
-            return;
-        }
-    }
-    float qx[NS][8];
-    fw_query<NS>(p, j, r, NS * dh, qx);                         // (on its way while the tiles are listed)
-    // ---- staging. f16: instruction x of a tile fills rows 8 (x & 3) .. + 7 of piece x >> 2; lane l brings
-    // the chunk that belongs at its place, (l % 8) ^ swz(row) of row l / 8
-    const int srow = 8 * (wave & 3) + (lane >> 3), ssrc = 16 * ((lane & 7) ^ fw_swz(srow));
-    auto dma_off = [&](int tile) { return min(srow, p.n_kv - 1 - (tile & FW_TILE) * FW_KT) * (int) p.k1 + ssrc; };
-    auto dma_src = [&](int tile) { return fw_src(j.kb + (size_t) ((tile & FW_TILE) * FW_KT) * p.k1); };
-    // instruction i of a wave: it keeps to one row group (wave & 3); of eight waves, two share one and halve its pieces
-    auto dma = [&](const FwSrc & src, int off, char * buf, int i) __attribute__((always_inline)) {
-        const int piece = NW == 8 ? min(2 * i + (wave >> 2), 8) : i;        // (piece 8 is brought twice)
-        fw_dma(src, off, 128 * piece, buf + piece * FW_PIECE + 1024 * (wave & 3));
-    };
-    // ---- the split's first tiles on their way while the tiles are listed; as a rule they are the list's.
-    // id[c]: the tile in slot c of the ring (-1: none)
-    char * const ring[4] = {t0, t1, t2, t3};
-    int id[RING];
-    auto dma_tile = [&](int tile, char * buf) __attribute__((always_inline)) {
-        const FwSrc src = dma_src(tile);
-        const int off = dma_off(tile);
-#pragma unroll
-        for (int i = 0; i < geo::DMA; ++i) dma(src, off, buf, i);
-    };
-    if constexpr (!QUANT) {
-#pragma unroll
-        for (int c = 0; c < RING - 1; ++c) if (c < j.nl) dma_tile(j.tile(p, c), ring[c]);
-    }
     FwTiles tiles;
     tiles.w0 = 0;
-    tiles.window<ROWS>(p, j);
-    bool listed = true;
+    int id0, id1;                                               // this tile, the next (-1: none)
+    if (wave < 4) {
+        float qx[NS][8];
+        fw_query<NS>(p, j, r, NS * dh, qx);
+        tiles.window<ROWS>(p, j);
+        id0 = tiles.next<ROWS>(p, j);
+        id1 = id0 >= 0 ? tiles.next<ROWS>(p, j) : -1;
+        wh8 qh[NS], ql[NS];
+        const float qsc = fw_terms<NS>(p, qx, qh, ql);          // of this half's part of the scores
+        const int kx0 = 128 * n16 + 16 * (g4 ^ fw_swz(n16)), kx1 = 128 * n16 + 16 * ((4 + g4) ^ fw_swz(n16));
+        const int ka0 = dh ? kx1 + 4 * FW_PIECE : kx0, ka1 = dh ? kx0 + 5 * FW_PIECE : kx1;
+        float m = -INFINITY, l = 0.f;
+        // the weights take V's steps before they are split, so they and O are held in units of 2^(qe - 7), 2^qe the
+        // largest step seen: neither term of a weight falls out of f16's range
+        int qe = -1000;
+        wf4 t[2];
+        auto scores = [&](const char * buf) __attribute__((always_inline)) {
+            wh8 a[AK + 1][2];
+            wh4 d[AK + 2][2];                                   // the blocks' steps of the lane's keys
+            wf4 x[2][2];
+            auto lda = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < RING - 1; ++c) {
-        id[c] = c == 0 || id[c - 1] >= 0 ? tiles.next<ROWS>(p, j) : -1;
-        listed &= id[c] < 0 || (id[c] & FW_TILE) == j.tile(p, c);
-    }
-    if constexpr (!QUANT) {
-        if (!listed) {
-            fw_vmcnt<0>();                                      // (behind the ones under way to the same places)
+                for (int u = 0; u < 2; ++u) {
+                    a[i % (AK + 1)][u] = *(const wh8 *) (buf + (i & 1 ? ka1 : ka0) + (i >> 1) * FW_PIECE + 2048 * u);
+                    d[i % (AK + 2)][u] = *(const wh4 *) (buf + 9 * FW_PIECE + 2 * ((NS * dh + i) * FW_KT + 16 * u + 4 * g4));
+                }
+            };
+            auto step = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int c = 0; c < RING - 1; ++c) if (id[c] >= 0) dma_tile(id[c], ring[c]);
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) t[u][c] = __builtin_fmaf((float) d[i % (AK + 2)][u][c], x[i & 1][u][c], t[u][c]);
+            };
+            t[0] = t[1] = wf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < AK; ++i) lda(i);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                if (i + AK < NS) lda(i + AK);
+                // one 32-block a step: its products are whole, then, a step later, take the block's step
+#pragma unroll
+                for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], wf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], x[i & 1][u], 0, 0, 0);
+                if (i) step(i - 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            step(NS - 1);
+            t[0] *= qsc;
+            t[1] *= qsc;
+            exch[wave][0][lane] = t[0];
+            exch[wave][1][lane] = t[1];
+        };
+        // the scores whole, the reference maximum, this wave's 16 keys' weights
+        auto softmax = [&](int tile, int slot) __attribute__((always_inline)) {
+            wf4 s[2] = {t[0] + exch[wave ^ 1][0][lane], t[1] + exch[wave ^ 1][1][lane]};
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, dtop[slot][i]);
+            if (p.softcap != 0.0f) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = p.softcap * tanhf(s[i >> 2][i & 3]);
+            }
+            if (tile >> 30) fw_mask(p, j, r, tile & FW_TILE, s);
+            float f = 1.f;
+            const int x = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : -1000;
+            if (x > qe) {                                       // the same in every wave; on the first tiles only
+                f = __builtin_amdgcn_ldexpf(1.f, max(qe - x, -200));
+                qe = x;
+            }
+            wf4 one[1] = {wf4{f, 0.f, 0.f, 0.f}};               // O's factor
+            const float ms = fw_raise<1>(s, m, l, one);
+            const float qf = qe == -1000 ? 1.f : __builtin_amdgcn_ldexpf(1.f, 7 - qe);
+            const wf4 sv = dh ? s[1] : s[0];
+            wf4 e;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], FW_L2E, ms));
+                l += e[i];
+            }
+            wgt[rg][dh][lane] = e * qf;
+            if (dh == 0 && g4 == 0) scl[rg][n16] = one[0][0];
+        };
+        fw_barrier();
+        for (int slot = 0; id0 >= 0; slot = slot == 2 ? 0 : slot + 1) {
+            scores(ring + slot * FQ_BUF);
+            fw_barrier();
+            softmax(id0, slot);
+            id0 = id1;
+            id1 = id1 >= 0 ? tiles.next<ROWS>(p, j) : -1;
+            fw_barrier();
         }
+        endl[rg][dh][lane] = l;
+        if (dh == 0) endm[rg][lane] = m;
+        if (wave == 0 && lane == 0) endq = qe;
+        fw_barrier();
+        return;
     }
-    id[RING - 1] = id[RING - 2] >= 0 ? tiles.next<ROWS>(p, j) : -1;         // fetched by the first body
-    wh8 qh[NS], ql[NS];
-    const float qsc = fw_terms<NS>(p, qx, qh, ql);              // of this half's part of the scores
-
+    tiles.window<ROWS>(p, j);
+    id0 = tiles.next<ROWS>(p, j);
+    id1 = id0 >= 0 ? tiles.next<ROWS>(p, j) : -1;
     wf4 o[ND];
-    float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = wf4{0.f, 0.f, 0.f, 0.f};
-    // quantised: the weights take V's steps before they are split, so they and O are held in units of
-    // 2^(qe - 7), 2^qe the largest step seen: neither term of a weight falls out of f16's range
-    int qe = -1000;
-
-    // per-lane LDS offsets: step i of this wave's half is step gs = 9 dh + i of the row, chunk g4 of half gs & 1 of piece gs >> 1
-    const int kx0 = 128 * n16 + 16 * (g4 ^ fw_swz(n16)), kx1 = 128 * n16 + 16 * ((4 + g4) ^ fw_swz(n16));
-    const int ka0 = dh ? kx1 + 4 * FW_PIECE : kx0, ka1 = dh ? kx0 + 5 * FW_PIECE : kx1;
     const int iq = (lane >> 2) & 3, ip = lane & 3, vrow = 4 * g4 + iq, vsw = fw_swz(vrow);
     int va[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) va[i] = (4 * dh + p.vpiece) * FW_PIECE + 128 * vrow + 16 * ((2 * i + (ip >> 1)) ^ vsw) + 8 * (ip & 1);
-
-    int par = 0;
-    wf4 s[2], t[2];                                             // the scores of the tile in hand, this half's of the next
-    float ms = 0.f, qf = 1.f;
-    wh8 ph[QUANT ? 2 : 1], pl[QUANT ? 2 : 1];                   // (quantised: a block's and the next one's)
+    const int vstep = 9 * FW_PIECE + 2 * ((8 * dh + 2 * p.vpiece) * FW_KT + 4 * g4);
+    wh8 v[AV + 1][2], ph[2], pl[2];                             // (terms of a block's weights, and of the next one's)
+    wh4 vd[AV + 1][2];
     float e[8];
-    // fragments from LDS are read AK (AV) steps ahead: with eight waves at it a read takes some 250 cycles, a step's
-    // matrix instructions 64. The first ones before the barrier's other business, and before the end of the scores
-    constexpr int AK = QUANT ? 2 : 4, AV = QUANT ? 2 : 3;
-    wh8 a[AK + 1][2], v[AV + 1][2];
-    wh4 ad[QUANT ? AK + 2 : 1][2], vd[QUANT ? AV + 1 : 1][2];   // quantised: their steps, of the lane's keys
-    auto lda = [&](const char * buf, int i) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) a[i % (AK + 1)][u] = *(const wh8 *) (buf + (i & 1 ? ka1 : ka0) + (i >> 1) * FW_PIECE + 2048 * u);
-        if constexpr (QUANT) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) ad[i % (AK + 2)][u] = *(const wh4 *) (buf + 9 * FW_PIECE + 2 * ((NS * dh + i) * FW_KT + 16 * u + 4 * g4));
-        }
-    };
     auto ldv = [&](const char * buf, int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) vd[b % (AV + 1)][u] = *(const wh4 *) (buf + vstep + 2 * (b * FW_KT + 16 * u));
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const char * a_ = buf + va[2 * (b & 1) + c] + (b >> 1) * FW_PIECE;
             const wh4 v0 = lds_tr4(a_), v1 = lds_tr4(a_ + 2048);
             v[b % (AV + 1)][c] = wh8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
         }
-        if constexpr (QUANT) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) vd[b % (AV + 1)][u] = *(const wh4 *) (buf + 9 * FW_PIECE + 2 * ((8 * dh + 2 * p.vpiece + b) * FW_KT + 16 * u + 4 * g4));
-        }
     };
-    // quantised: the weights times V's steps of 32-block b, as two terms
+    auto ahead = [&](const char * buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < AV; ++b) ldv(buf, b);
+    };
+    // the weights times V's steps of 32-block b, as two terms
     auto terms = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
@@ -620,97 +861,13 @@ __global__ __launch_bounds__((FlGeo<KV, RG>::NT), (FlGeo<KV, RG>::NT / 256)) voi
             split2p(e[i], (float) d[i & 3], e[i + 1], (float) d[(i & 3) + 1], i, ph[b & 1], pl[b & 1]);
         }
     };
-    auto ahead = [&](const char * buf) __attribute__((always_inline)) {
+    // O^T += V^T P^T, 32-blocks b0 .. b1 - 1 of this wave's channels
+    auto values = [&](const char * buf, const int b0, const int b1) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < AK; ++i) lda(buf, i);
-    };
-    // this half's part of the scores of the tile in `buf` to the exchange; meanwhile (W) the weights of the tile in
-    // hand, whose values lie in `vbuf`
-    // and a further tile goes to `fbuf`: instruction by instruction here, where the matrix unit hides them (all at once
-    // behind the barrier they took 800 cycles). They run on past the last tile, into places no longer read
-    auto scores = [&](const char * buf, const char * vbuf, char * fbuf, const FwSrc & fsrc, int foff, auto with) __attribute__((always_inline)) {
-        constexpr bool W = decltype(with)::value;
-        t[0] = t[1] = wf4{0.f, 0.f, 0.f, 0.f};
-        wf4 tl[2] = {t[0], t[0]};                               // a chain of its own for the low term
-        wf4 x[2][2];
-        auto step = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) t[u][c] = __builtin_fmaf((float) ad[i % (AK + 2)][u][c], x[i & 1][u][c], t[u][c]);
-        };
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            if constexpr (W && !QUANT) { if (i < geo::DMA) dma(fsrc, foff, fbuf, i); }
-            if (i + AK < NS) lda(buf, i + AK);
-            if (W && i >= NS - AV) ldv(vbuf, i - (NS - AV));
-            if constexpr (!QUANT) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], t[u], 0, 0, 0);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) tl[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], tl[u], 0, 0, 0);
-            } else {
-                // one 32-block a step: its products are whole, then, a step later, take the block's step
-#pragma unroll
-                for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], wf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], x[i & 1][u], 0, 0, 0);
-                if (i) step(i - 1);
-            }
-            if constexpr (W) {
-                if (i < 8) {
-                    e[i] = fw_weight(s, i, ms);
-                    l += e[i];
-                    if constexpr (QUANT) e[i] *= qf;
-                    else if (i & 1) split2(e[i - 1], e[i], i - 1, ph[0], pl[0]);
-                } else if constexpr (QUANT) terms(0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if constexpr (!QUANT) { t[0] += tl[0]; t[1] += tl[1]; }
-        else step(NS - 1);
-        t[0] *= qsc;
-        t[1] *= qsc;
-        exch[par][wave][0][lane] = t[0];
-        exch[par][wave][1][lane] = t[1];
-    };
-    // behind the barrier: the scores of tile `tile` (slot C) whole, the reference maximum; the first fragments of the
-    // tile in `buf` meanwhile
-    auto whole = [&](int tile, const int C, const char * buf) __attribute__((always_inline)) {
-        const wf4 x0 = exch[par][wave ^ 1][0][lane], x1 = exch[par][wave ^ 1][1][lane];
-        __builtin_amdgcn_sched_barrier(0);
-        ahead(buf);
-        s[0] = t[0] + x0;
-        s[1] = t[1] + x1;
-        par ^= 1;
-        if (p.softcap != 0.0f) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = p.softcap * tanhf(s[i >> 2][i & 3]);
-        }
-        if (tile >> 30) fw_mask(p, j, r, tile & FW_TILE, s);
-        if constexpr (QUANT) {
-            float top = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, dtop[C][i]);
-            const int x = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : -1000;
-            if (x > qe) {                                       // the same in every wave; on the first tiles only
-                const float f = __builtin_amdgcn_ldexpf(1.f, max(qe - x, -200));
-#pragma unroll
-                for (int d = 0; d < ND; ++d) o[d] *= f;
-                qe = x;
-            }
-            qf = qe == -1000 ? 1.f : __builtin_amdgcn_ldexpf(1.f, 7 - qe);
-        }
-        ms = fw_raise<ND>(s, m, l, o);
-    };
-    // O^T += V^T P^T: keys 4 g4 + 0..3 of the two 16-key blocks a lane, as the scores lie; 32 channels at a
-    // time, so that a term's product does not wait for the other's
-    auto values = [&](const char * buf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int b = 0; b < ND / 2; ++b) {
+        for (int b = b0; b < b1; ++b) {
             if (b + AV < ND / 2) ldv(buf, b + AV);
-            if constexpr (QUANT) { if (b + 1 < ND / 2) terms(b + 1); }          // a 32-block of V: its steps enter the weights
-            const int w = QUANT ? b & 1 : 0;
+            if (b + 1 < ND / 2) terms(b + 1);
+            const int w = b & 1;
             o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], ph[w], o[2 * b], 0, 0, 0);
             o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], ph[w], o[2 * b + 1], 0, 0, 0);
             o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], pl[w], o[2 * b], 0, 0, 0);
@@ -718,63 +875,41 @@ __global__ __launch_bounds__((FlGeo<KV, RG>::NT), (FlGeo<KV, RG>::NT / 256)) voi
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // the tile in slot C, its scores in hand, with the next tile's scores on the way: the weights are taken among the
-    // matrix instructions of the next tile's scores, the exchange passes under this tile's values. The barrier then
-    // frees slot C (and tells that the tile after the next is whole)
-    auto body = [&](auto slot_) __attribute__((always_inline)) {
-        constexpr int C = decltype(slot_)::value, C1 = (C + 1) % RING, F = (C + RING - 1) % RING;
-        const int further = id[F] >= 0 ? id[F] : id[C];         // (behind the last tile: any, into a place no longer read)
-        scores(ring[C1], ring[C], ring[F], dma_src(further), dma_off(further), std::true_type{});
-        values(ring[C]);
-        if constexpr (!QUANT) fw_vmcnt<(RING - 3) * geo::DMA>();    // the tile after the next has landed
-        fw_barrier();
-        id[C] = id[F] >= 0 ? tiles.next<ROWS>(p, j) : -1;
-        whole(id[C1], C1, ring[(C + 2) % RING]);                // (fragments read for nothing where no such tile is left)
+    auto weights = [&]() __attribute__((always_inline)) {
+        const wf4 e0 = wgt[rg][0][lane], e1 = wgt[rg][1][lane];
+        const float f = scl[rg][n16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = i < 4 ? e0[i & 3] : e1[i & 3];
+        if (__any(f != 1.f)) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= f;
+        }
+        terms(0);
     };
-
-    if constexpr (!QUANT) fw_vmcnt<0>();
-    __syncthreads();
-    if (id[0] >= 0) {
-        ahead(t0);
-        scores(t0, t0, nullptr, dma_src(id[0]), 0, std::false_type{});
+    fw_barrier();
+    if (id0 >= 0) {
         fw_barrier();
-        whole(id[0], 0, t1);
-        const char * last;
-        for (;;) {
-            last = t0;
-            if (id[1] < 0) break;
-            body(std::integral_constant<int, 0>{});
-            last = t1;
-            if (id[2] < 0) break;
-            body(std::integral_constant<int, 1>{});
-            last = t2;
-            if (id[3 % RING] < 0) break;
-            body(std::integral_constant<int, 2>{});
-            if constexpr (RING == 4) {
-                last = t3;
-                if (id[0] < 0) break;
-                body(std::integral_constant<int, 3>{});
-            }
+        ahead(ring);
+        fw_barrier();
+        for (int slot = 0;;) {                                  // the tile in `slot`; beside it the next one's scores
+            const char * buf = ring + slot * FQ_BUF;
+            weights();
+            values(buf, 0, ND / 4);
+            if (id1 >= 0) fw_barrier();
+            values(buf, ND / 4, ND / 2);
+            if (id1 < 0) break;
+            id1 = tiles.next<ROWS>(p, j);
+            slot = slot == 2 ? 0 : slot + 1;
+            ahead(ring + slot * FQ_BUF);
+            fw_barrier();
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            e[i] = fw_weight(s, i, ms);
-            l += e[i];
-            if constexpr (QUANT) e[i] *= qf;
-            else if (i & 1) split2(e[i - 1], e[i], i - 1, ph[0], pl[0]);
-        }
-        if constexpr (!QUANT) fw_vmcnt<0>();                    // no DMA outlives the workgroup's LDS
-#pragma unroll
-        for (int b = 0; b < AV; ++b) ldv(last, b);
-        if constexpr (QUANT) terms(0);
-        values(last);
     }
-    if constexpr (QUANT) {
-        const float f = qe == -1000 ? 1.f : __builtin_amdgcn_ldexpf(1.f, qe - 7);
+    fw_barrier();
+    const int qe = endq;
+    const float f = qe == -1000 ? 1.f : __builtin_amdgcn_ldexpf(1.f, qe - 7);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] *= f;
-    }
-    fw_store<576, 512, KV, ND>(p, j, j.kb, p.k1, 64 * p.vpiece, j.r0 + 16 * rg, 256 * dh, m, l, o);
+    for (int d = 0; d < ND; ++d) o[d] *= f;
+    fw_store<576, 512, KV, ND>(p, j, j.kb, p.k1, 64 * p.vpiece, j.r0 + 16 * rg, 256 * dh, endm[rg][lane], endl[rg][0][lane] + endl[rg][1][lane], o);
 }
 
 // ---- expanded: K rows of 192, V rows of 128 ----------------------------------------------------------
@@ -1167,10 +1302,10 @@ void fa_wide_run(OpCtx & c, ggml_tensor * dst) {
         if (pl.rows == 32) k_fattn_expanded<1, 2><<<grid, 128, 0, c.st>>>(a);
         else if (pl.rows == 64) k_fattn_expanded<1, 4><<<grid, 256, 0, c.st>>>(a);
         else        k_fattn_expanded<2, 4><<<grid, 256, 0, c.st>>>(a);
-    } else if (k->type == GGML_TYPE_Q8_0) k_fattn_latent<GGML_TYPE_Q8_0, 2><<<grid, FlGeo<GGML_TYPE_Q8_0, 2>::NT, 0, c.st>>>(a);
-    else if (k->type == GGML_TYPE_Q4_0) k_fattn_latent<GGML_TYPE_Q4_0, 2><<<grid, FlGeo<GGML_TYPE_Q4_0, 2>::NT, 0, c.st>>>(a);
-    else if (pl.rows == 32) k_fattn_latent<GGML_TYPE_F16, 2><<<grid, FlGeo<GGML_TYPE_F16, 2>::NT, 0, c.st>>>(a);
-    else k_fattn_latent<GGML_TYPE_F16, 4><<<grid, FlGeo<GGML_TYPE_F16, 4>::NT, 0, c.st>>>(a);
+    } else if (k->type == GGML_TYPE_Q8_0) k_fattn_latent_q<GGML_TYPE_Q8_0><<<grid, 768, 0, c.st>>>(a);
+    else if (k->type == GGML_TYPE_Q4_0) k_fattn_latent_q<GGML_TYPE_Q4_0><<<grid, 768, 0, c.st>>>(a);
+    else if (pl.rows == 32) k_fattn_latent<2><<<grid, FlGeo<2>::NT, 0, c.st>>>(a);
+    else k_fattn_latent<4><<<grid, FlGeo<4>::NT, 0, c.st>>>(a);
     if (pl.nsplit > 1) {
         const unsigned rows = (unsigned) (a.S * a.n_q * a.H), chunks = (unsigned) (DV / std::min(DV, 256));
         if (rows * (size_t) chunks >= FW_JOIN_ROWS) {

@@ -596,7 +596,7 @@ def test_sharp_scores(ctx, backend):
 
 @pytest.mark.parametrize("form", FORMS)
 def test_replayed_graph(ctx, backend, form):
-    """the same graph again and again, new inputs between (its replays are captured), other work between them"""
+    """the same graph again and again, new inputs between, other work between them"""
     c = Case(ctx, **sized(form))
     first = c.run(backend)
     g = ctx.build(c.out)
@@ -614,6 +614,37 @@ def test_replayed_graph(ctx, backend, form):
             assert rel(y, c.want()) < ATT_REL
             c.q = keep
     assert rel(first, want) < ATT_REL
+
+
+def test_captured_graphs(pkg, backend):
+    """graphs of enough nodes to be captured, replayed in turn: they share the stream's workspace. Smaller ones run as they are"""
+    cases = []
+    for i, kw in enumerate((dict(heads=32, m=3000), dict(heads=16, n=20, m=500, cache="q4_0"), dict(form="expanded", heads=8, n=40, m=300))):
+        c = Case(pkg.Context(), seed=i, **kw)
+        y = c.out
+        for f in (2.0, 0.5, 4.0, 0.25):
+            y = c.ctx.scale(y, f)
+        c.y, c.big, c.small = y, c.ctx.build(y), c.ctx.build(c.out)
+        c.ctx.alloc(backend)
+        for t, a in c.feeds:
+            t.set(a)
+        cases.append(c)
+    before = backend.stats()["graph_replay"]
+    for c in cases:
+        for _ in range(3):
+            c.ctx.compute(backend, c.small)
+        c.first = c.out.numpy().reshape(c.shape)
+        assert rel(c.first, c.want()) < ATT_REL
+    assert backend.stats()["graph_replay"] == before
+    for i in range(6):
+        for c in cases:
+            if i % 2:
+                c.ctx.compute(backend, c.small)
+            c.ctx.compute(backend, c.big)
+            assert np.array_equal(c.y.numpy().reshape(c.shape), c.first)
+    assert backend.stats()["graph_replay"] >= before + 12          # (the first pass runs, the second may record)
+    for c in cases:
+        c.ctx.free()
 
 
 def test_two_backends_at_once(pkg, backend):
