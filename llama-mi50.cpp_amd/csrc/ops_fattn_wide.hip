@@ -68,10 +68,10 @@ __device__ __forceinline__ void split2(float x0, float x1, int j, wh8 & hi, wh8 
     hi[j] = h[0]; hi[j + 1] = h[1];
     lo[j] = l[0]; lo[j + 1] = l[1];
 }
-// the same of the products x0 d0, x1 d1: the remainder of the whole product
-__device__ __forceinline__ void split2p(float x0, float d0, float x1, float d1, int j, wh8 & hi, wh8 & lo) {
-    const wh2 h = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(x0, d0, 0.f), __builtin_fmaf(x1, d1, 0.f)));   // (d f16: mixed FMAs)
-    const wh2 l = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(x0, d0, -(float) h[0]), __builtin_fmaf(x1, d1, -(float) h[1])));
+// the same of the products x0 d0, x1 d1, h being x0 and x1 to f16: the high terms multiplied there, the remainder of the whole product
+__device__ __forceinline__ void split2p(float x0, float x1, wh2 h, wh2 d, int j, wh8 & hi, wh8 & lo) {
+    h *= d;
+    const wh2 l = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(x0, (float) d[0], -(float) h[0]), __builtin_fmaf(x1, (float) d[1], -(float) h[1])));
     hi[j] = h[0]; hi[j + 1] = h[1];
     lo[j] = l[0]; lo[j + 1] = l[1];
 }
@@ -617,7 +617,8 @@ __global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
 // Two barriers a tile: behind the halves of the scores, and behind the weights. A tile on every CU at once, 4 bits: 2.6 us
 // with all of it in one wave a SIMD, 2.2 with the last kind apart, 2.1 so; alone on the chip 2.6, 1.8 and 1.7. What is left
 // is the vector unit's: 600 instructions a SIMD and tile, 5 cycles each (the matrix unit's 68 take 1100 cycles beside them)
-constexpr int FQ_BUF = 9 * FW_PIECE + 18 * FW_KT * 2;           // a tile and its blocks' steps, [block][key] f16
+constexpr int FQ_BUF = 9 * FW_PIECE + 18 * FW_KT * 2;           // a tile and its blocks' steps, [block][key] f16, ...
+constexpr int FQ_STEP = 10;                                     // ... times 2^10, out of the range where f16 keeps few bits
 
 // the last kind: blocks through registers, two tiles ahead of the store
 template <int KV, int ROWS>
@@ -633,43 +634,49 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
     for (int c = 0; c < 4; ++c) at[c] = rot * FW_PIECE + 128 * row + 16 * ((4 * (x8 & 1) + ((c + rot) & 3)) ^ sw);
 #pragma unroll
     for (int c = 0; c < NL; ++c) from[c] = x8 * QB + 2 + 8 * ((c + rot) & (NL - 1));
-    const int nib0 = rot & 2 ? 4 : 0, nib1 = (rot + 1) & 2 ? 4 : 0;            // 4 bits: shifts of chunks 0 and 1; 2 and 3 have the others
-    struct Regs { uint2 a[2][NL], w; uint16_t d[3]; } set[2];
+    // integers to f16 exactly: 1024 + b has the byte b in its low bits, two at a time. 8 bits: b is n + 128; 4 bits: n + 8,
+    // or 16 times that, from the high nibbles, so a chunk's nibble is a mask, a factor and an offset
+    struct Nib { uint32_t mask; wh2 mul, off; };
+    auto nibble = [](bool high) {
+        const _Float16 m = high ? 0.0625f : 1.f, o = high ? -72.f : -1032.f;
+        return Nib{high ? 0xF0F0F0F0u : 0x0F0F0F0Fu, wh2{m, m}, wh2{o, o}};
+    };
+    const Nib n0 = nibble(rot & 2), n1 = nibble((rot + 1) & 2), n2 = nibble(!(rot & 2)), n3 = nibble(!((rot + 1) & 2)), pnib = nibble(pval & 16);
+    struct Regs { uint2 a[2][NL], w; _Float16 d[3]; } set[2];
     auto load = [&](int tile, Regs & q) __attribute__((always_inline)) {
         const char * kr = j.kb + (size_t) min((tile & FW_TILE) * FW_KT + row, p.n_kv - 1) * p.k1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            q.d[i] = ld_u16(kr + (x8 + 8 * i) * QB);
+            __builtin_memcpy(&q.d[i], kr + (x8 + 8 * i) * QB, 2);
 #pragma unroll
             for (int c = 0; c < NL; ++c) __builtin_memcpy(&q.a[i][c], kr + from[c] + 8 * i * QB, 8);
         }
         const char * b = kr + pblk * QB;
-        q.d[2] = ld_u16(b);
+        __builtin_memcpy(&q.d[2], b, 2);
         __builtin_memcpy(&q.w, b + 2 + (KV == GGML_TYPE_Q8_0 ? pval : pval & 15), 8);
     };
-    // integers to f16 exactly: 1024 + n has n in its low bits, two at a time. Bytes 2t, 2t + 1 of u (n + 128; n + 8)
-    auto pair = [](uint32_t u, int t) __attribute__((always_inline)) {
-        const _Float16 off = KV == GGML_TYPE_Q8_0 ? 1152.f : 1032.f;
-        const uint32_t pr = __builtin_amdgcn_perm(0x64646464u, u, t ? 0x04030402u : 0x04010400u);
-        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(wh2, pr) - wh2{off, off});
+    auto pair = [](uint32_t u, int t, const Nib & k) __attribute__((always_inline)) {      // bytes 2t, 2t + 1 of u
+        const wh2 x = __builtin_bit_cast(wh2, __builtin_amdgcn_perm(0x64646464u, u, t ? 0x04030402u : 0x04010400u));
+        return __builtin_bit_cast(uint32_t, KV == GGML_TYPE_Q8_0 ? x - wh2{(_Float16) 1152.f, (_Float16) 1152.f} : __builtin_elementwise_fma(x, k.mul, k.off));
     };
-    // a chunk: 8 values from 8 bytes, or from their nibbles at bit `sh`
-    auto chunk = [&](uint2 u, int sh) __attribute__((always_inline)) {
-        const uint32_t x = KV == GGML_TYPE_Q8_0 ? u.x ^ 0x80808080u : u.x >> sh & 0x0F0F0F0Fu, y = KV == GGML_TYPE_Q8_0 ? u.y ^ 0x80808080u : u.y >> sh & 0x0F0F0F0Fu;
-        return make_uint4(pair(x, 0), pair(x, 1), pair(y, 0), pair(y, 1));
+    auto chunk = [&](uint2 u, const Nib & k) __attribute__((always_inline)) {              // 8 values
+        const uint32_t x = KV == GGML_TYPE_Q8_0 ? u.x ^ 0x80808080u : u.x & k.mask, y = KV == GGML_TYPE_Q8_0 ? u.y ^ 0x80808080u : u.y & k.mask;
+        return make_uint4(pair(x, 0, k), pair(x, 1, k), pair(y, 0, k), pair(y, 1, k));
     };
     auto store = [&](const Regs & q, int slot, int half) __attribute__((always_inline)) {
         char * const buf = ring + slot * FQ_BUF;
-        uint16_t * const steps = (uint16_t *) (buf + 9 * FW_PIECE);
-        steps[(x8 + 8 * half) * FW_KT + row] = q.d[half];
+        _Float16 * const steps = (_Float16 *) (buf + 9 * FW_PIECE);
+        steps[(x8 + 8 * half) * FW_KT + row] = q.d[half] * (_Float16) (1 << FQ_STEP);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-            *(uint4 *) (buf + at[c] + 4 * half * FW_PIECE) = chunk(q.a[half][c & (NL - 1)], c == 0 ? nib0 : c == 1 ? nib1 : c == 2 ? 4 - nib0 : 4 - nib1);
-        if (half == 0) return;
-        steps[pblk * FW_KT + row] = q.d[2];
-        *(uint4 *) (buf + 8 * FW_PIECE + 128 * row + 16 * (x8 ^ sw)) = chunk(q.w, pval & 16 ? 4 : 0);
-        const float top = wave_max<64>(fmaxf(fmaxf(fabsf(h2f(q.d[0])), fabsf(h2f(q.d[1]))), fabsf(h2f(q.d[2]))));
-        if (lane == 0) dtop[slot][wave] = top;
+            *(uint4 *) (buf + at[c] + 4 * half * FW_PIECE) = chunk(q.a[half][c & (NL - 1)], c == 0 ? n0 : c == 1 ? n1 : c == 2 ? n2 : n3);
+        if (half == 0) {
+            const float top = wave_max<64>(fmaxf(fmaxf(fabsf((float) q.d[0]), fabsf((float) q.d[1])), fabsf((float) q.d[2])));
+            if (lane == 0) dtop[slot][wave] = top;
+            return;
+        }
+        steps[pblk * FW_KT + row] = q.d[2] * (_Float16) (1 << FQ_STEP);
+        *(uint4 *) (buf + 8 * FW_PIECE + 128 * row + 16 * (x8 ^ sw)) = chunk(q.w, pnib);
     };
 
     // the split's first two tiles on their way while the tiles are listed; as a rule they are the list's
@@ -721,6 +728,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
     const int n16 = lane & 15, g4 = lane >> 4, rg = wave >> 1 & 1, dh = wave & 1;
     const FwJob j = fw_job<ROWS, false>(p);
     if (wave >= 8) {
+        __builtin_amdgcn_s_setprio(2);                          // (the longest of the three; without it 49 us instead of 47)
         fw_produce<KV, ROWS>(p, j, ring, dtop);
         return;
     }
@@ -735,13 +743,14 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
         id0 = tiles.next<ROWS>(p, j);
         id1 = id0 >= 0 ? tiles.next<ROWS>(p, j) : -1;
         wh8 qh[NS], ql[NS];
-        const float qsc = fw_terms<NS>(p, qx, qh, ql);          // of this half's part of the scores
+        const float qsc = fw_terms<NS>(p, qx, qh, ql) * (1.f / (1 << FQ_STEP));        // of this half's part of the scores
         const int kx0 = 128 * n16 + 16 * (g4 ^ fw_swz(n16)), kx1 = 128 * n16 + 16 * ((4 + g4) ^ fw_swz(n16));
         const int ka0 = dh ? kx1 + 4 * FW_PIECE : kx0, ka1 = dh ? kx0 + 5 * FW_PIECE : kx1;
         float m = -INFINITY, l = 0.f;
         // the weights take V's steps before they are split, so they and O are held in units of 2^(qe - 7), 2^qe the
-        // largest step seen: neither term of a weight falls out of f16's range
-        int qe = -1000;
+        // largest (scaled) step seen, 1 at least: weights, up to 2^8, and their products with steps stay in f16's range.
+        // A step of 64 or more is infinite here: rows that see one are computed again
+        int qe = 0;
         wf4 t[2];
         auto scores = [&](const char * buf) __attribute__((always_inline)) {
             wh8 a[AK + 1][2];
@@ -792,14 +801,14 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
             }
             if (tile >> 30) fw_mask(p, j, r, tile & FW_TILE, s);
             float f = 1.f;
-            const int x = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : -1000;
+            const int x = top < INFINITY ? __builtin_amdgcn_frexp_expf(top) + FQ_STEP : 0;
             if (x > qe) {                                       // the same in every wave; on the first tiles only
-                f = __builtin_amdgcn_ldexpf(1.f, max(qe - x, -200));
+                f = __builtin_amdgcn_ldexpf(1.f, qe - x);
                 qe = x;
             }
             wf4 one[1] = {wf4{f, 0.f, 0.f, 0.f}};               // O's factor
             const float ms = fw_raise<1>(s, m, l, one);
-            const float qf = qe == -1000 ? 1.f : __builtin_amdgcn_ldexpf(1.f, 7 - qe);
+            const float qf = __builtin_amdgcn_ldexpf(1.f, 7 - qe);
             const wf4 sv = dh ? s[1] : s[0];
             wf4 e;
 #pragma unroll
@@ -839,6 +848,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
     wh8 v[AV + 1][2], ph[2], pl[2];                             // (terms of a block's weights, and of the next one's)
     wh4 vd[AV + 1][2];
     float e[8];
+    wh2 eh[4];
     auto ldv = [&](const char * buf, int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) vd[b % (AV + 1)][u] = *(const wh4 *) (buf + vstep + 2 * (b * FW_KT + 16 * u));
@@ -858,7 +868,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             const wh4 d = vd[b % (AV + 1)][i >> 2];
-            split2p(e[i], (float) d[i & 3], e[i + 1], (float) d[(i & 3) + 1], i, ph[b & 1], pl[b & 1]);
+            split2p(e[i], e[i + 1], eh[i >> 1], wh2{d[i & 3], d[(i & 3) + 1]}, i, ph[b & 1], pl[b & 1]);
         }
     };
     // O^T += V^T P^T, 32-blocks b0 .. b1 - 1 of this wave's channels
@@ -880,6 +890,8 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
         const float f = scl[rg][n16];
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = i < 4 ? e0[i & 3] : e1[i & 3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) eh[i] = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(e[2 * i], e[2 * i + 1]));
         if (__any(f != 1.f)) {
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= f;
@@ -905,8 +917,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
         }
     }
     fw_barrier();
-    const int qe = endq;
-    const float f = qe == -1000 ? 1.f : __builtin_amdgcn_ldexpf(1.f, qe - 7);
+    const float f = __builtin_amdgcn_ldexpf(1.f, endq - 7 - FQ_STEP);
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] *= f;
     fw_store<576, 512, KV, ND>(p, j, j.kb, p.k1, 64 * p.vpiece, j.r0 + 16 * rg, 256 * dh, endm[rg][lane], endl[rg][0][lane] + endl[rg][1][lane], o);

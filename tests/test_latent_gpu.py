@@ -579,7 +579,7 @@ def test_magnitudes(ctx, backend, q_scale, spread, scale):
 
 
 @pytest.mark.parametrize("cache", ["q8_0", "q4_0"])
-@pytest.mark.parametrize("spread", [1e-4, 40.0])
+@pytest.mark.parametrize("spread", [1e-4, 40.0, 2e4])   # (2e5 would pass f16's range in a 4-bit step)
 def test_magnitudes_of_steps(ctx, backend, cache, spread):
     """quantised rows far from 1, and rows whose steps differ by thousands: the first tiles small, later ones large"""
     c = Case(ctx, cache=cache, heads=16, n=2, m=300, spread=spread, scale=192 ** -0.5 / spread)
