@@ -644,16 +644,17 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
     const Nib n0 = nibble(rot & 2), n1 = nibble((rot + 1) & 2), n2 = nibble(!(rot & 2)), n3 = nibble(!((rot + 1) & 2)), pnib = nibble(pval & 16);
     struct Regs { uint2 a[2][NL], w; _Float16 d[3]; } set[2];
     auto load = [&](int tile, Regs & q) __attribute__((always_inline)) {
-        const char * kr = j.kb + (size_t) min((tile & FW_TILE) * FW_KT + row, p.n_kv - 1) * p.k1;
+        const int key0 = (tile & FW_TILE) * FW_KT;
+        const char * kb = j.kb + (size_t) key0 * p.k1;          // (uniform; a lane's offset has 32 bits)
+        const uint32_t kr = (uint32_t) min(row, p.n_kv - 1 - key0) * (uint32_t) p.k1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            __builtin_memcpy(&q.d[i], kr + (x8 + 8 * i) * QB, 2);
+            __builtin_memcpy(&q.d[i], kb + (kr + x8 * QB) + 8 * i * QB, 2);
 #pragma unroll
-            for (int c = 0; c < NL; ++c) __builtin_memcpy(&q.a[i][c], kr + from[c] + 8 * i * QB, 8);
+            for (int c = 0; c < NL; ++c) __builtin_memcpy(&q.a[i][c], kb + (kr + from[c]) + 8 * i * QB, 8);
         }
-        const char * b = kr + pblk * QB;
-        __builtin_memcpy(&q.d[2], b, 2);
-        __builtin_memcpy(&q.w, b + 2 + (KV == GGML_TYPE_Q8_0 ? pval : pval & 15), 8);
+        __builtin_memcpy(&q.d[2], kb + (kr + pblk * QB), 2);
+        __builtin_memcpy(&q.w, kb + (kr + pblk * QB + (KV == GGML_TYPE_Q8_0 ? pval : pval & 15)) + 2, 8);
     };
     auto pair = [](uint32_t u, int t, const Nib & k) __attribute__((always_inline)) {      // bytes 2t, 2t + 1 of u
         const wh2 x = __builtin_bit_cast(wh2, __builtin_amdgcn_perm(0x64646464u, u, t ? 0x04030402u : 0x04010400u));
@@ -702,9 +703,12 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
         if (t0 < 0) return false;
         if (t1 >= 0) store(q, slot, 0);
         fw_barrier();
-        if (t1 >= 0) store(q, slot, 1);
-        const int t3 = t2 >= 0 ? tiles.next<ROWS>(p, j) : -1;
-        if (t3 >= 0) load(t3, q);
+        int t3 = -1;
+        if (t1 >= 0) {
+            store(q, slot, 1);
+            if (t2 >= 0) t3 = tiles.next<ROWS>(p, j);
+            if (t3 >= 0) load(t3, q);
+        }
         t0 = t1; t1 = t2; t2 = t3;
         slot = slot == 2 ? 0 : slot + 1;
         fw_barrier();
