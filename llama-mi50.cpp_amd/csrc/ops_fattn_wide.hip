@@ -949,24 +949,35 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     tiles.w0 = 0;
     tiles.window<ROWS>(p, j);
     const int srow = lane >> 3, ssrc = 16 * ((lane & 7) ^ fw_swz(8 * wave + srow));   // (W is even: the same for rb below)
-    auto dma = [&](int tile, char * buf) {
+    struct Src { FwSrc k, v; int ko[4 / W], vo[4 / W]; };
+    auto source = [&](int tile) __attribute__((always_inline)) {
         const int key0 = (tile & FW_TILE) * FW_KT;
-        const FwSrc ks = fw_src(j.kb + (size_t) key0 * p.k1), vs = fw_src(vb + (size_t) key0 * p.v1);
+        Src q{fw_src(j.kb + (size_t) key0 * p.k1), fw_src(vb + (size_t) key0 * p.v1)};
 #pragma unroll
         for (int b = 0; b < 4 / W; ++b) {
-            const int rb = wave + W * b, row = min(8 * rb + srow, p.n_kv - 1 - key0);   // eight rows
-            const int ko = row * (int) p.k1 + ssrc, vo = row * (int) p.v1 + ssrc;
-#pragma unroll
-            for (int i = 0; i < 5; ++i) fw_dma(i < 3 ? ks : vs, i < 3 ? ko : vo, 128 * (i < 3 ? i : i - 3), buf + i * FW_PIECE + 1024 * rb);
+            const int row = min(8 * (wave + W * b) + srow, p.n_kv - 1 - key0);  // eight rows
+            q.ko[b] = row * (int) p.k1 + ssrc;
+            q.vo[b] = row * (int) p.v1 + ssrc;
         }
+        return q;
+    };
+    auto dma = [&](const Src & q, char * buf, int i) __attribute__((always_inline)) {      // piece i
+#pragma unroll
+        for (int b = 0; b < 4 / W; ++b)
+            fw_dma(i < 3 ? q.k : q.v, i < 3 ? q.ko[b] : q.vo[b], 128 * (i < 3 ? i : i - 3), buf + i * FW_PIECE + 1024 * (wave + W * b));
     };
     char * const ring[3] = {t0, t1, t2};
     int id[3];
     id[0] = tiles.next<ROWS>(p, j);
     id[1] = id[0] >= 0 ? tiles.next<ROWS>(p, j) : -1;
     id[2] = -1;
-    if (id[0] >= 0) dma(id[0], t0);
-    if (id[1] >= 0) dma(id[1], t1);
+    if (id[0] >= 0) {
+        const Src q0 = source(id[0]), q1 = source(id[1] >= 0 ? id[1] : id[0]);
+#pragma unroll
+        for (int i = 0; i < 5; ++i) dma(q0, t0, i);
+#pragma unroll
+        for (int i = 0; i < 5; ++i) dma(q1, t1, i);
+    }
 
     wh8 qh[NT][NS], ql[NT][NS];
     float qsc[NT], m[NT], l[NT];
@@ -987,10 +998,12 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     auto body = [&](auto slot_) __attribute__((always_inline)) {
         constexpr int C = decltype(slot_)::value, F = (C + 2) % 3, N = (C + 1) % 3;
         char * const buf = ring[C];
-        if (id[N] >= 0) fw_vmcnt<DMA>(); else fw_vmcnt<0>();    // this wave's part of the tile
+        fw_vmcnt<DMA>();                                        // this wave's part of the tile
         fw_barrier();                                           // the tile is whole; the one before it is free
+        // the tile after the next on its way, a piece a step below (all at once they hold the wave up); behind the last
+        // one any, into a place no longer read
         id[F] = id[N] >= 0 ? tiles.next<ROWS>(p, j) : -1;
-        if (id[F] >= 0) dma(id[F], ring[F]);
+        const Src q = source(id[F] >= 0 ? id[F] : id[C]);
         wf4 s[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = wf4{0.f, 0.f, 0.f, 0.f};
@@ -1004,6 +1017,7 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             if (i + 2 < NS) lda(i + 2);
+            if (i < 5) dma(q, ring[F], i);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -1067,6 +1081,7 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
         if (id[2] < 0) break;
         body(std::integral_constant<int, 2>{});
     }
+    fw_vmcnt<0>();                                              // no DMA outlives the workgroup's LDS
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) fw_store<192, 128, GGML_TYPE_F16, ND>(p, j, vb, p.v1, 0, rg0 + 16 * nt, 0, m[nt], l[nt], o[nt]);
 }
@@ -1213,7 +1228,7 @@ constexpr int FW_MAP_TOK = 17;   // from so many tokens on the tile map is built
 struct FwRows { int rows; double t1, t2; };
 static FwPlan fw_plan(const ggml_tensor * dst) {
     const ggml_tensor * q = dst->src[0], * k = dst->src[1], * v = dst->src[2], * m = dst->src[3];
-    static const FwRows latent[2] = {{32, 1.33, 0}, {64, 1.63, 0}}, quant[1] = {{32, 1.8, 0}}, expanded[3] = {{32, 1.03, 1.27}, {64, 0.93, 1.46}, {128, 1.45, 2.8}};
+    static const FwRows latent[2] = {{32, 1.33, 0}, {64, 1.63, 0}}, quant[1] = {{32, 1.55, 0}}, expanded[3] = {{32, 1.03, 1.27}, {64, 0.93, 1.46}, {128, 1.45, 2.8}};
     FwPlan p{};
     p.wide = k->ne[0] == 576;
     const int64_t G = q->ne[2] / k->ne[2], nrow = q->ne[1] * G, units = k->ne[2] * q->ne[3];
