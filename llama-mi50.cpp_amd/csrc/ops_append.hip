@@ -43,6 +43,8 @@ template <typename T, int V> __device__ __forceinline__ void stv(T * p, const Pa
 // channel pair (a, b) of a head: a at i and b at i + np, or (ADJ) neighbours. V pairs a step: 16-byte
 // loads and stores when rows and pair counts allow them. In place is safe: a thread reads the pair it
 // writes. 64-bit angle arithmetic costs ~100 instructions a pair and is spent once a token, not once a head.
+// Memory bounds the long ones: 4096 tokens of 32 heads of 128 in f16, 67 MB in 13.5 us (5.0 TB/s; a large copy 5.2); 1521
+// tokens of 16 heads of 80 in f32 5.4 us; one token 2.5 us, a launch.
 template <typename T, bool ADJ, int V>
 __global__ __launch_bounds__(256) void k_rope_axes(const char * __restrict__ x, const int32_t * __restrict__ pos, const float * __restrict__ ff,
                                                    char * __restrict__ y, G4 gx, G4 gy, RopeP p, int np, int hper) {
@@ -213,7 +215,8 @@ void op_concat(OpCtx & c, ggml_tensor * dst) {
 // A row is [normalised part | rotated heads] or the reverse (a latent cache), or rotated heads alone
 // (keys); a second, unturned row (values) may go to a cache of its own. The row is assembled in LDS in
 // 32 bits and rounded once into the cache's type. Against the separate launches (RMS_NORM + MUL, ROPE,
-// CONCAT, SET_ROWS) it saves their round trips through memory, and at a token or two the launches.
+// CONCAT, SET_ROWS) it saves their round trips through memory, and at a token or two the launches. The chain fetch, sum,
+// rotate, store of a row bounds it: 8 latent rows 5.2 us, 2011 7.3 us (7 MB), 512 rows of keys and of values 5.8 us.
 // ---------------------------------------------------------------------------
 struct RowDst {
     char * base; size_t nb1; int64_t ne1; int type;             // a cache

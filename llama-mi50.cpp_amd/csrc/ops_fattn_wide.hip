@@ -10,10 +10,10 @@
 // Precision: the result is f32 and callers ask for GGML_PREC_F32, so nothing is rounded to 11 bits on
 // the way: q (scaled by a power of two into f16's range) and the softmax weights enter the f16 matrix
 // units as two terms, high + low (22 bits), each product twice; K and V are exact in f16, quantised
-// ones as their integers with the block's step applied in f32 (to the products of K, to the weights of
-// V). The rate that bounds the large cases is therefore half the f16 rate.
+// ones as their integers: a block's step is applied in f32 to the products of K, and to the weights of V
+// as their terms are formed. The rate that bounds the large cases is therefore half the f16 rate.
 //
-// Both kernels: S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_16x16x32_f16, so a lane holds scores and
+// All kernels: S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_16x16x32_f16, so a lane holds scores and
 // outputs of one query row (lane & 15): softmax state and rescaling are lane-local, and P^T goes from
 // the score registers straight into the second product (its k index runs over the keys the lane has;
 // V's rows follow by transposing LDS reads). Query rows of one KV head are flattened token-major, so a
@@ -291,6 +291,9 @@ __device__ __forceinline__ float fw_weight(const wf4 (&s)[2], int i, float ms) {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], FW_L2E, ms));
 }
 
+// a sink's part of the denominator; one of -inf beside a row that sees nothing is no NaN
+__device__ __forceinline__ float fw_sink(float sink, float m) { return sink == m ? 1.f : __builtin_amdgcn_exp2f((sink - m) * FW_L2E); }
+
 // A row key by key, leaving masked keys out: an infinity or a NaN in V times a weight of 0 is a NaN, and
 // what lies in the rows of hidden keys may not reach the result, so a row that shows one is computed
 // again by its wave. acc[c]: channel d0 + 64 c + lane
@@ -370,7 +373,7 @@ __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, cons
         if (p.sinks) {
             const float sk = p.sinks[hd], mm = fmaxf(m, sk);
             a = m == mm ? 1.f : __builtin_amdgcn_exp2f((m - mm) * FW_L2E);
-            l = l * a + __builtin_amdgcn_exp2f((sk - mm) * FW_L2E);
+            l = l * a + fw_sink(sk, mm);
         }
         const float inv = l == 0.f ? 0.f : a / l;
         char * out = p.dst + (size_t) hd * p.d1 + (size_t) tk * p.d2 + (size_t) j.seq * p.d3 + 4 * (d0 + 4 * g4);
@@ -392,6 +395,10 @@ __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, cons
 // much for one wave beside the rest of it, so the pair shares: wave dh multiplies channels [288 dh, + 288)
 // of the keys, the halves of the scores are exchanged through LDS (the only barrier of a tile), both do
 // the softmax, and each keeps half of the output channels.
+// Few rows (RG = 2): the cache bounds it. 4 sequences of up to 32768 tokens, 32 heads: 38 us for 123.5 MB, 6 TB/s while it
+// streams (a large copy 5.2), 4 us before and 2 behind, the join 6. Many (RG = 4): the matrix unit and its power. 512
+// tokens, 32 heads, 4096 keys: 250 us warm, 1.08 PFLOP/s of f16 products (a large library product 1.18); a build of
+// 14 % fewer busy cycles took the same time at a clock lower by as much
 template <int RG> struct FlGeo {
     static constexpr int NT = 128 * RG;                         // threads
     // tiles in the ring, three ahead of the one in use where they fit beside the exchange
@@ -615,8 +622,9 @@ __global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
 //   4 waves   values of this tile, half of the channels of a row group each
 //   4 waves   blocks of the tile after the next into f16 integers
 // Two barriers a tile: behind the halves of the scores, and behind the weights. A tile on every CU at once, 4 bits: 2.6 us
-// with all of it in one wave a SIMD, 2.2 with the last kind apart, 2.1 so; alone on the chip 2.6, 1.8 and 1.7. What is left
-// is the vector unit's: 600 instructions a SIMD and tile, 5 cycles each (the matrix unit's 68 take 1100 cycles beside them)
+// with all of it in one wave a SIMD, 2.2 with the last kind apart, 1.9 so; alone on the chip 2.6, 1.8 and 1.5 (8 bits 1.65).
+// 4 x 32768 tokens at 4 bits: 40 us for 34.7 MB, 250 before the kinds were parted and the steps read ahead. What is left is
+// the chain of one tile: 500 vector instructions and 68 matrix instructions a SIMD, 2000 and 1100 of some 3800 cycles
 constexpr int FQ_BUF = 9 * FW_PIECE + 18 * FW_KT * 2;           // a tile and its blocks' steps, [block][key] f16, ...
 constexpr int FQ_STEP = 10;                                     // ... times 2^10, out of the range where f16 keeps few bits
 
@@ -928,8 +936,10 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
 }
 
 // ---- expanded: K rows of 192, V rows of 128 ----------------------------------------------------------
-// W waves of NT row groups of 16 each: a K or V fragment from LDS serves NT groups (and both terms), so
-// with NT = 2 the LDS moves half of what the matrix instructions could take.
+// W waves of NT row groups of 16 each, two workgroups a CU: a K or V fragment from LDS serves NT groups (and both terms),
+// so with NT = 2 the LDS moves half of what the matrix instructions could take. 2048 tokens, 32 heads, 4096 keys: 260 us
+// warm, 0.98 PFLOP/s, bounded as above; 499 tokens on 512: 23 us, the 16 tiles of the longest rows one after another, 1 us
+// each (a tile's scores under the last one's weights, as above: 0.85, but 5 % lost on 2048 tokens, where NT = 2 did not fit)
 template <int NT, int W>
 __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     constexpr int NS = 6, ND = 8, ROWS = 16 * NT * W, BUF = 5 * FW_PIECE, DMA = 20 / W;
@@ -1087,7 +1097,8 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
 }
 
 // Joins the splits of one row. A workgroup takes CH channels, four of them a lane; its lane groups (waves) take every
-// GR-th split, so eight loads of 16 bytes a lane are in flight. The partials come from L2 / Infinity Cache.
+// GR-th split, so eight loads of 16 bytes a lane are in flight. The partials come from L2 / Infinity Cache: 128 rows, 64
+// splits, 16.8 MB in 6 us.
 template <int DV>
 __global__ __launch_bounds__(256) void k_fattn_wide_join(FwArgs p) {
     constexpr int CH = DV < 256 ? DV : 256, LG = CH / 4, GR = 256 / LG;     // channels, lanes and groups of them
@@ -1112,7 +1123,7 @@ __global__ __launch_bounds__(256) void k_fattn_wide_join(FwArgs p) {
     const float w = none ? 0.f : ms == m ? 1.f : __builtin_amdgcn_exp2f((ms - m) * FW_L2E);
     wgt[tid] = none ? -1.f : w;
     float l = block_sum(ls * w, red);
-    if (p.sinks) l += __builtin_amdgcn_exp2f((p.sinks[h] - m) * FW_L2E);
+    if (p.sinks) l += fw_sink(p.sinks[h], m);
     __syncthreads();
     wf4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = g; s0 < p.nsplit; s0 += 8 * GR) {
@@ -1175,7 +1186,7 @@ __global__ __launch_bounds__(256) void k_fattn_wide_join_rows(FwArgs p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 32, 64);
     }
-    if (p.sinks) l += __builtin_amdgcn_exp2f((sink - m) * FW_L2E);
+    if (p.sinks) l += fw_sink(sink, m);
     if (g) return;
     const size_t t = id / p.H % p.n_q, seq = id / ((size_t) p.H * p.n_q);
     const float inv = l == 0.f ? 0.f : 1.f / l;

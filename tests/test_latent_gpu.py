@@ -558,6 +558,21 @@ def test_sinks(ctx, backend, form, m):
     assert rel(c.run(backend), c.want(sinks=sinks)) < ATT_REL
 
 
+@pytest.mark.parametrize("form,n,m", [("latent", 1, 40), ("latent", 3, 900), ("latent", 80, 900), ("expanded", 3, 40), ("expanded", 3, 900), ("expanded", 300, 900)])
+def test_sinks_of_minus_infinity(ctx, backend, form, n, m):
+    """add nothing, and leave a row that sees nothing 0: without splits, and with each of the joins"""
+    def mask(rng, S, H, n, m):
+        v = np.where(rng.random((S, 1, n, m)) < 0.3, -np.inf, 0).astype(np.float16)
+        v[1, :, 0] = -np.inf
+        return v
+    c = Case(ctx, form=form, heads=8, n=n, m=m, S=2, mask=mask)
+    ts = ctx.new_tensor("f32", 8)
+    c.out.raw.src[4] = ts.ptr
+    c.feeds.append((ts, np.full(8, -np.inf, np.float32)))
+    y = c.run(backend)
+    assert not y[1, 0].any() and rel(y, c.want()) < ATT_REL
+
+
 @pytest.mark.parametrize("cache", ["f16", "q8_0", "q4_0"])
 @pytest.mark.parametrize("heads,n,m", [(8, 2, 200), (64, 3, 150)])
 def test_values_behind_the_rotated_channels(ctx, backend, cache, heads, n, m):
