@@ -42,7 +42,7 @@ constexpr int FW_PIECE = FW_KT * 128;        // 64 channels of a tile in LDS, f1
 constexpr int FW_TB = 32;                    // tokens of one entry of the mask's tile map
 constexpr int FW_MAX_SPLIT = 256;
 constexpr int FW_TILE = 0x3FFFFFFF;          // a listed tile's number; bit 30: the mask or the row's end cuts it
-constexpr float FW_L2E = 1.4426950408889634f;
+constexpr float FW_L2E = 1.4426950408889634f;   // scores, masks and sinks are taken to base 2 where they come in
 enum { FW_LIVE = 1, FW_MIXED = 2 };          // tile map bits: some key is visible; some mask value is not 0
 
 struct FwArgs {
@@ -55,7 +55,7 @@ struct FwArgs {
     float * opart, * mpart, * lpart;         // [nsplit][S * n_q * H][DV | 1 | 1]
     const uint8_t * map; int n_tb;           // [mne3][n_tb][n_tiles] tile map, or null
     int n_q, n_kv, H, G, Hkv, S, nsplit, n_tiles, vpiece;   // vpiece: 64s of channels of a K row before V
-    float scale, softcap, max_bias, m0, m1f;
+    float scale, softcap, max_bias, m0, m1f;   // to base 2: softcap, or scale where there is none
     uint32_t n_head_log2;
 };
 
@@ -122,8 +122,9 @@ template <int KV> __device__ __forceinline__ float fw_get(const char * row, int 
     else return dequant_one<KV>(row + (size_t) (i >> 5) * qsize_of<KV>(), i & 31);
 }
 
+// the factor of the mask
 __device__ __forceinline__ float fw_slope(const FwArgs & p, uint32_t h) {
-    return p.max_bias > 0.0f ? (h < p.n_head_log2 ? powf(p.m0, h + 1) : powf(p.m1f, 2 * (h - p.n_head_log2) + 1)) : 1.0f;
+    return p.max_bias > 0.0f ? FW_L2E * (h < p.n_head_log2 ? powf(p.m0, h + 1) : powf(p.m1f, 2 * (h - p.n_head_log2) + 1)) : FW_L2E;
 }
 
 // What a workgroup works on: rows [r0, r0 + ROWS) of KV head hk of sequence seq, row r being token r / G
@@ -271,28 +272,28 @@ __device__ __forceinline__ void fw_mask(const FwArgs & p, const FwJob & j, int r
 }
 
 // Online softmax of a lane's row over its 8 keys of the tile and the other three lanes' (the row lies in
-// four). First the reference maximum: raised only when a score exceeds it by 5.5 (weights up to 2^8), so
-// O is rescaled on the first tiles only. Returns -m log2(e) for the weights e^(s - m).
+// four). First the reference maximum: raised only when a score exceeds it by 8 (weights up to 2^8), so
+// O is rescaled on the first tiles only. Returns -m for the weights 2^(s - m).
 template <int ND>
 __device__ __forceinline__ float fw_raise(const wf4 (&s)[2], float & m, float & l, wf4 (&o)[ND]) {
     float mt = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     mt = fw_row4<false>(mt);
-    const bool raise = mt > m + 5.5f;                           // false while nothing was visible
+    const bool raise = mt > m + 8.f;                            // false while nothing was visible
     if (__any(raise)) {
-        const float al = raise ? __builtin_amdgcn_exp2f((m - mt) * FW_L2E) : 1.f;
+        const float al = raise ? __builtin_amdgcn_exp2f(m - mt) : 1.f;
         if (raise) m = mt;
         l *= al;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= al;
     }
-    return m == -INFINITY ? 0.f : -m * FW_L2E;
+    return m == -INFINITY ? 0.f : -m;
 }
 __device__ __forceinline__ float fw_weight(const wf4 (&s)[2], int i, float ms) {
-    return __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], FW_L2E, ms));
+    return __builtin_amdgcn_exp2f(s[i >> 2][i & 3] + ms);
 }
 
 // a sink's part of the denominator; one of -inf beside a row that sees nothing is no NaN
-__device__ __forceinline__ float fw_sink(float sink, float m) { return sink == m ? 1.f : __builtin_amdgcn_exp2f((sink - m) * FW_L2E); }
+__device__ __forceinline__ float fw_sink(float sink, float m) { return sink == m ? 1.f : __builtin_amdgcn_exp2f(sink - m); }
 
 // A row key by key, leaving masked keys out: an infinity or a NaN in V times a weight of 0 is a NaN, and
 // what lies in the rows of hidden keys may not reach the result, so a row that shows one is computed
@@ -322,8 +323,8 @@ __device__ __forceinline__ void fw_again(const FwArgs & p, const FwJob & j, cons
             x += mv;
         }
         const float mn = fmaxf(m, wave_max<64>(x));
-        const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * FW_L2E);
-        const float e = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x - mn) * FW_L2E);
+        const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        const float e = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - mn);
         m = mn;
         l = l * al + wave_sum<64>(e);
 #pragma unroll
@@ -371,8 +372,8 @@ __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, cons
     if (p.nsplit == 1) {
         float a = 1.f;
         if (p.sinks) {
-            const float sk = p.sinks[hd], mm = fmaxf(m, sk);
-            a = m == mm ? 1.f : __builtin_amdgcn_exp2f((m - mm) * FW_L2E);
+            const float sk = p.sinks[hd] * FW_L2E, mm = fmaxf(m, sk);
+            a = m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm);
             l = l * a + fw_sink(sk, mm);
         }
         const float inv = l == 0.f ? 0.f : a / l;
@@ -825,7 +826,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
             wf4 e;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], FW_L2E, ms));
+                e[i] = __builtin_amdgcn_exp2f(sv[i] + ms);
                 l += e[i];
             }
             wgt[rg][dh][lane] = e * qf;
@@ -1118,12 +1119,13 @@ __global__ __launch_bounds__(256) void k_fattn_wide_join(FwArgs p) {
     float ms = -INFINITY, ls = 0.f;                             // a thread a split
     if (tid < p.nsplit) { ms = p.mpart[tid * rows + id]; ls = p.lpart[tid * rows + id]; }
     float m = block_max(ms, red);
-    if (p.sinks) m = fmaxf(m, p.sinks[h]);
+    const float sink = p.sinks ? p.sinks[h] * FW_L2E : -INFINITY;
+    m = fmaxf(m, sink);
     const bool none = ms == -INFINITY && ls == 0.f;
-    const float w = none ? 0.f : ms == m ? 1.f : __builtin_amdgcn_exp2f((ms - m) * FW_L2E);
+    const float w = none ? 0.f : ms == m ? 1.f : __builtin_amdgcn_exp2f(ms - m);
     wgt[tid] = none ? -1.f : w;
     float l = block_sum(ls * w, red);
-    if (p.sinks) l += fw_sink(p.sinks[h], m);
+    if (p.sinks) l += fw_sink(sink, m);
     __syncthreads();
     wf4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = g; s0 < p.nsplit; s0 += 8 * GR) {
@@ -1154,7 +1156,7 @@ __global__ __launch_bounds__(256) void k_fattn_wide_join_rows(FwArgs p) {
     const size_t rows = (size_t) p.S * p.n_q * p.H, id = (size_t) blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= rows) return;
     const int h = (int) (id % p.H);
-    const float sink = p.sinks ? p.sinks[h] : -INFINITY;
+    const float sink = p.sinks ? p.sinks[h] * FW_L2E : -INFINITY;
     float m = sink;
     for (int s = lane; s < p.nsplit; s += 64) m = fmaxf(m, p.mpart[s * rows + id]);
     m = wave_max<64>(m);
@@ -1176,7 +1178,7 @@ __global__ __launch_bounds__(256) void k_fattn_wide_join_rows(FwArgs p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (!(ms[i] == -INFINITY && ls[i] == 0.f)) {        // a split that saw nothing left nothing to read
-                const float w = ms[i] == m ? 1.f : __builtin_amdgcn_exp2f((ms[i] - m) * FW_L2E);
+                const float w = ms[i] == m ? 1.f : __builtin_amdgcn_exp2f(ms[i] - m);
                 l += ls[i] * w;
                 o += v[i] * w;
             }
@@ -1320,7 +1322,8 @@ void fa_wide_run(OpCtx & c, ggml_tensor * dst) {
     a.scale = mx_op_param<float>(dst, 0);
     a.max_bias = mx_op_param<float>(dst, 1);
     a.softcap = mx_op_param<float>(dst, 2);
-    if (a.softcap != 0.0f) a.scale /= a.softcap;
+    if (a.softcap != 0.0f) { a.scale /= a.softcap; a.softcap *= FW_L2E; }
+    else a.scale *= FW_L2E;
     a.n_head_log2 = 1u << (uint32_t) floor(log2((double) a.H));
     a.m0 = powf(2.0f, -(a.max_bias) / a.n_head_log2);
     a.m1f = powf(2.0f, -(a.max_bias / 2.0f) / a.n_head_log2);
