@@ -216,7 +216,8 @@ void op_concat(OpCtx & c, ggml_tensor * dst) {
 // (keys); a second, unturned row (values) may go to a cache of its own. The row is assembled in LDS in
 // 32 bits and rounded once into the cache's type. Against the separate launches (RMS_NORM + MUL, ROPE,
 // CONCAT, SET_ROWS) it saves their round trips through memory, and at a token or two the launches. The chain fetch, sum,
-// rotate, store of a row bounds it: 8 latent rows 5.2 us, 2011 7.3 us (7 MB), 512 rows of keys and of values 5.8 us.
+// rotate, store of a row bounds it: 8 latent rows 5.1 us, 2011 6.5 us (7 MB), 512 rows of keys and of values 5.4 us; 1800 rows of
+// 16 heads of keys and of values in f32, 59 MB, 14.6 us.
 // ---------------------------------------------------------------------------
 struct RowDst {
     char * base; size_t nb1; int64_t ne1; int type;             // a cache
@@ -227,7 +228,7 @@ struct AppendP {
     const char * nx; size_t n_tok; const float * nw; char * nout; size_t nout_tok; int n_norm, norm_at; float eps;   // n_norm = 0: none
     const char * rx; size_t r_head, r_tok; const int32_t * pos; const float * ff; int heads, dim, rot_at, np, adj; int64_t ntok;
     RopeP rope;
-    const char * vx; size_t v_tok;
+    const char * vx; size_t v_tok; int v4;                      // v4: rows of whole 16 bytes, aligned
     RowDst k, v;
 };
 constexpr int APPEND_MAX_ROW = 8192;                            // elements of both rows in LDS: 32 KB
@@ -244,7 +245,11 @@ __device__ __forceinline__ void store_row(const RowDst & d, const float * row, i
     const int nt = blockDim.x;
     switch (d.type) {                                           // uniform
         case GGML_TYPE_F32:
-            for (int i = threadIdx.x; i < d.width; i += nt) ((float *) o)[i] = row[i];
+            if ((((uintptr_t) o) & 15) == 0 && d.width % 4 == 0) {
+                for (int i = 4 * threadIdx.x; i < d.width; i += 4 * nt) *(float4 *) (o + 4 * i) = *(const float4 *) (row + i);
+            } else {
+                for (int i = threadIdx.x; i < d.width; i += nt) ((float *) o)[i] = row[i];
+            }
             break;
         case GGML_TYPE_F16:
         case GGML_TYPE_BF16: {
@@ -271,6 +276,8 @@ __device__ __forceinline__ void store_row(const RowDst & d, const float * row, i
     }
 }
 
+// LATENT: the normalised part, no second row
+template <bool LATENT>
 __global__ __launch_bounds__(256) void k_append_rows(AppendP p) {
     extern __shared__ __align__(16) float row[];                // [k.width, to a multiple of 4][v.width]
     const int v0 = (p.k.width + 3) & ~3;
@@ -279,9 +286,10 @@ __global__ __launch_bounds__(256) void k_append_rows(AppendP p) {
     const int64_t t = blockIdx.x;
     const int nt = blockDim.x, tid = threadIdx.x;
     // everything the row needs is fetched first, up to AHEAD elements (pairs) a thread; a chain of table, sum and
-    // rotation that fetched its own spent 9 us on 2011 latent rows, 7 of them waiting
+    // rotation that fetched its own spent 9 us on 2011 latent rows, 7 of them waiting (and one kernel for both kinds of row 7.2: registers)
     constexpr int AHEAD = 4;
-    float nv[AHEAD], vv[AHEAD], r0[AHEAD], r1[AHEAD];
+    float nv[LATENT ? AHEAD : 1], wv[LATENT ? AHEAD : 1], r0[AHEAD], r1[AHEAD];
+    float4 vv[LATENT ? 1 : AHEAD];                              // (four elements each where p.v4 says so, else .x)
     const float * xn = (const float *) (p.nx + t * p.n_tok), * xv = (const float *) (p.vx + t * p.v_tok);
     const int pairs = p.heads * p.np;
     auto pair = [&](int u, float & x0, float & x1) {
@@ -293,13 +301,19 @@ __global__ __launch_bounds__(256) void k_append_rows(AppendP p) {
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
         const int i = tid + a * nt;
-        nv[a] = i < p.n_norm ? xn[i] : 0.f;
-        vv[a] = i < p.v.width ? xv[i] : 0.f;
+        if constexpr (LATENT) {
+            nv[a] = i < p.n_norm ? xn[i] : 0.f;
+            wv[a] = i < p.n_norm ? p.nw[i] : 0.f;
+        } else {
+            vv[a] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p.v4) { if (4 * i < p.v.width) vv[a] = ((const float4 *) xv)[i]; }
+            else if (i < p.v.width) vv[a].x = xv[i];
+        }
         if (i < pairs) pair(i, r0[a], r1[a]);
     }
-    const int64_t kcell = cell_of(p.k, t), vcell = p.v.width ? cell_of(p.v, t) : -1;
+    const int64_t kcell = cell_of(p.k, t), vcell = !LATENT && p.v.width ? cell_of(p.v, t) : -1;
     for (int i = tid; i < p.np; i += nt) tab[i] = rope_pair(p.rope, i, p.pos, t, p.ntok, p.ff);
-    if (p.n_norm) {
+    if constexpr (LATENT) {
         float s = 0.f;
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) s += nv[a] * nv[a];
@@ -307,18 +321,23 @@ __global__ __launch_bounds__(256) void k_append_rows(AppendP p) {
         s = block_sum(s, red);
         const float inv = 1.0f / sqrtf(s / p.n_norm + p.eps);
         float * out = p.nout ? (float *) (p.nout + t * p.nout_tok) : nullptr;
-        auto put = [&](int i, float x) {
-            const float v = x * inv * p.nw[i];
+        auto put = [&](int i, float x, float w) {
+            const float v = x * inv * w;
             row[p.norm_at + i] = v;
             if (out) out[i] = v;
         };
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) if (tid + a * nt < p.n_norm) put(tid + a * nt, nv[a]);
-        for (int i = tid + AHEAD * nt; i < p.n_norm; i += nt) put(i, xn[i]);
-    }
+        for (int a = 0; a < AHEAD; ++a) if (tid + a * nt < p.n_norm) put(tid + a * nt, nv[a], wv[a]);
+        for (int i = tid + AHEAD * nt; i < p.n_norm; i += nt) put(i, xn[i], p.nw[i]);
+    } else if (p.v4) {
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) if (tid + a * nt < p.v.width) row[v0 + tid + a * nt] = vv[a];
-    for (int i = tid + AHEAD * nt; i < p.v.width; i += nt) row[v0 + i] = xv[i];
+        for (int a = 0; a < AHEAD; ++a) if (4 * (tid + a * nt) < p.v.width) *(float4 *) (row + v0 + 4 * (tid + a * nt)) = vv[a];
+        for (int i = tid + AHEAD * nt; 4 * i < p.v.width; i += nt) *(float4 *) (row + v0 + 4 * i) = ((const float4 *) xv)[i];
+    } else {
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) if (tid + a * nt < p.v.width) row[v0 + tid + a * nt] = vv[a].x;
+        for (int i = tid + AHEAD * nt; i < p.v.width; i += nt) row[v0 + i] = xv[i];
+    }
     __syncthreads();                                            // the table
     auto turn = [&](int u, float x0, float x1) {
         const int h = u / p.np, i = u % p.np;
@@ -341,7 +360,7 @@ __global__ __launch_bounds__(256) void k_append_rows(AppendP p) {
     }
     __syncthreads();
     store_row(p.k, row, kcell);
-    store_row(p.v, row + v0, vcell);
+    if constexpr (!LATENT) store_row(p.v, row + v0, vcell);
 }
 
 static const ggml_tensor * through_views(const ggml_tensor * t) {
@@ -450,6 +469,7 @@ int fuse_append_rows(OpCtx & c, ggml_cgraph * g, int i, const UseCount & use_map
         fused_io_ok({sk, sv}, {x, rope->src[1], rope->src[2], sk->src[1], sv->src[0], sv->src[1]})) {
         const ggml_tensor * vx = sv->src[0];
         p.vx = (const char *) vx->data; p.v_tok = vx->nb[1];
+        p.v4 = p.v.width % 4 == 0 && ((uintptr_t) vx->data | vx->nb[1]) % 16 == 0;
         last = at[2];
     } else { sv = nullptr; p.v.width = 0; }
     if (!sv && !fused_io_ok({sk, keep_mul ? mul : nullptr}, {x, rope->src[1], rope->src[2], sk->src[1], nx, w})) return 0;
@@ -462,7 +482,8 @@ int fuse_append_rows(OpCtx & c, ggml_cgraph * g, int i, const UseCount & use_map
     const size_t lds = (size_t) (p.k.width + 3 + p.v.width) * sizeof(float);
     const int threads = p.k.width + p.v.width >= 1024 ? 256 : p.k.width + p.v.width >= 512 ? 192 : 64;
     MX_KLOG("append_rows norm=%d heads=%d dim=%d mode=%d type=%d v=%d keep=%d", p.n_norm, p.heads, p.dim, p.rope.mode, p.k.type, p.v.width, (int) keep_mul);
-    k_append_rows<<<(unsigned) ntok, threads, lds, c.st>>>(p);
+    if (cat) k_append_rows<true><<<(unsigned) ntok, threads, lds, c.st>>>(p);
+    else     k_append_rows<false><<<(unsigned) ntok, threads, lds, c.st>>>(p);
     return last - i + 1;
 }
 
