@@ -397,7 +397,7 @@ __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, cons
 // of the keys, the halves of the scores are exchanged through LDS (the only barrier of a tile), both do
 // the softmax, and each keeps half of the output channels.
 // Few rows (RG = 2): the cache bounds it. 4 sequences of up to 32768 tokens, 32 heads: 38 us for 123.5 MB, 6 TB/s while it
-// streams (a large copy 5.2), 4 us before and 2 behind, the join 6. Many (RG = 4): the matrix unit and its power. 512
+// streams (a large copy 5.2), 4 us before and 2 behind, the join 5.4. Many (RG = 4): the matrix unit and its power. 512
 // tokens, 32 heads, 4096 keys: 250 us warm, 1.08 PFLOP/s of f16 products (a large library product 1.18); a build of
 // 14 % fewer busy cycles took the same time at a clock lower by as much
 template <int RG> struct FlGeo {
@@ -1097,16 +1097,15 @@ __global__ __launch_bounds__(64 * W, W / 2) void k_fattn_expanded(FwArgs p) {
     for (int nt = 0; nt < NT; ++nt) fw_store<192, 128, GGML_TYPE_F16, ND>(p, j, vb, p.v1, 0, rg0 + 16 * nt, 0, m[nt], l[nt], o[nt]);
 }
 
-// Joins the splits of one row. A workgroup takes CH channels, four of them a lane; its lane groups (waves) take every
-// GR-th split, so eight loads of 16 bytes a lane are in flight. The partials come from L2 / Infinity Cache: 128 rows, 64
-// splits, 16.8 MB in 6 us.
+// Joins the splits of one row. A workgroup takes 128 channels, four of them a lane; its eight half waves take every eighth
+// split, so eight loads of 16 bytes a lane are in flight, on their way while every wave computes the weights for itself.
+// The partials come from L2 / Infinity Cache: 128 rows, 64 splits, 16.8 MB in 5.4 us (with 256 channels and the weights
+// by the workgroup 6.0).
 template <int DV>
 __global__ __launch_bounds__(256) void k_fattn_wide_join(FwArgs p) {
-    constexpr int CH = DV < 256 ? DV : 256, LG = CH / 4, GR = 256 / LG;     // channels, lanes and groups of them
-    __shared__ float wgt[FW_MAX_SPLIT];
-    __shared__ float red[16];
+    constexpr int CH = 128, LG = CH / 4, GR = 256 / LG;         // channels, lanes and groups of them
     __shared__ __align__(16) wf4 part[GR][LG];
-    const int tid = threadIdx.x, c = tid % LG, g = tid / LG;
+    const int tid = threadIdx.x, lane = tid & 63, c = tid % LG, g = tid / LG;
     const size_t rows = (size_t) p.S * p.n_q * p.H, id = blockIdx.x;
     const int h = (int) (id % p.H);
     const float * src = p.opart + id * DV + blockIdx.y * CH + 4 * c;
@@ -1115,25 +1114,34 @@ __global__ __launch_bounds__(256) void k_fattn_wide_join(FwArgs p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = *(const wf4 *) (src + (size_t) min(s0 + i * GR, p.nsplit - 1) * rows * DV);
     };
-    fetch(g);                                                   // on their way while the weights are computed
-    float ms = -INFINITY, ls = 0.f;                             // a thread a split
-    if (tid < p.nsplit) { ms = p.mpart[tid * rows + id]; ls = p.lpart[tid * rows + id]; }
-    float m = block_max(ms, red);
+    fetch(g);
+    constexpr int NQ = FW_MAX_SPLIT / 64;                       // split 64 q + lane
+    float ms[NQ], ls[NQ], w[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const int s = 64 * q + lane;
+        ms[q] = s < p.nsplit ? p.mpart[s * rows + id] : -INFINITY;
+        ls[q] = s < p.nsplit ? p.lpart[s * rows + id] : 0.f;
+    }
     const float sink = p.sinks ? p.sinks[h] * FW_L2E : -INFINITY;
-    m = fmaxf(m, sink);
-    const bool none = ms == -INFINITY && ls == 0.f;
-    const float w = none ? 0.f : ms == m ? 1.f : __builtin_amdgcn_exp2f(ms - m);
-    wgt[tid] = none ? -1.f : w;
-    float l = block_sum(ls * w, red);
+    const float m = fmaxf(wave_max<64>(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]))), sink);
+    float l = 0.f;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const bool none = ms[q] == -INFINITY && ls[q] == 0.f;
+        w[q] = none ? -1.f : ms[q] == m ? 1.f : __builtin_amdgcn_exp2f(ms[q] - m);
+        if (!none) l += ls[q] * w[q];
+    }
+    l = wave_sum<64>(l);
     if (p.sinks) l += fw_sink(sink, m);
-    __syncthreads();
     wf4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = g; s0 < p.nsplit; s0 += 8 * GR) {
-        if (s0 != g) fetch(s0);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        if (64 * q >= p.nsplit) break;
+        if (q) fetch(64 * q + g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int s = s0 + i * GR;
-            const float a = s < p.nsplit ? wgt[s] : -1.f;
+            const float a = __shfl(w[q], g + i * GR, 64);       // (splits past the last have none)
             if (!(a < 0.f)) o += v[i] * a;
         }
     }
@@ -1357,7 +1365,7 @@ void fa_wide_run(OpCtx & c, ggml_tensor * dst) {
             if (pl.wide) k_fattn_wide_join_rows<512><<<grid, 256, 0, c.st>>>(a);
             else         k_fattn_wide_join_rows<128><<<grid, 256, 0, c.st>>>(a);
         } else {
-            const dim3 grid(rows, chunks);
+            const dim3 grid(rows, (unsigned) (DV / 128));
             if (pl.wide) k_fattn_wide_join<512><<<grid, 256, 0, c.st>>>(a);
             else         k_fattn_wide_join<128><<<grid, 256, 0, c.st>>>(a);
         }
