@@ -73,6 +73,10 @@ struct ggml_tensor * mxg_rope_multi_back(mxg_context * ctx, struct ggml_tensor *
 /* a and b joined along dim 0..3 (ggml_concat); their other dimensions and types agree, else NULL */
 struct ggml_tensor * mxg_concat(mxg_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b, int dim);
 struct ggml_tensor * mxg_soft_max_ext(mxg_context * ctx, struct ggml_tensor * a, struct ggml_tensor * mask, float scale, float max_bias);
+/* softmax(scale q k^T [softcap] + mask) v (ggml_flash_attn_ext). q f32 [DK, n_q, heads, seqs], k [DK, n_kv, kv heads, seqs or 1],
+ * v [DV, ...]; mask f16 [>= n_kv, >= n_q, 1 or heads, 1 or seqs] or NULL; the result is f32 [DV, heads, n_q, seqs]. Keys wider than
+ * the values (latent attention): DK 576 with v the first 512 channels of k's own rows, or those behind its first 64 (a view of
+ * the same tensor; f16, q8_0, q4_0), and DK 192 with DV 128 (f16). f16 rows lie on 16 bytes. Other such widths: NULL. */
 struct ggml_tensor * mxg_flash_attn_ext(mxg_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k, struct ggml_tensor * v,
                                         struct ggml_tensor * mask, float scale, float max_bias, float logit_softcap);
 struct ggml_tensor * mxg_argsort(mxg_context * ctx, struct ggml_tensor * a, enum ggml_sort_order order);

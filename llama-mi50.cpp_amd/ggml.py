@@ -233,6 +233,8 @@ class Context:
         return self._t(self.lib.mxg_soft_max_ext(self.ptr, a.ptr, self._p(mask), scale, max_bias))
 
     def flash_attn_ext(self, q, k, v, mask, scale, max_bias=0.0, softcap=0.0):
+        """softmax(scale q k^T + mask) v (ggml_flash_attn_ext). Keys wider than the values are latent attention: 576 with v the
+        first 512 channels of k's rows, or those behind the first 64, as a view of the same cache (f16, q8_0, q4_0); 192 and 128 (f16)."""
         return self._t(self.lib.mxg_flash_attn_ext(self.ptr, q.ptr, k.ptr, v.ptr, self._p(mask), scale, max_bias, softcap))
 
     def argsort(self, a, desc=False):
