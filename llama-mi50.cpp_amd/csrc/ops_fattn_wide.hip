@@ -1238,7 +1238,11 @@ __global__ __launch_bounds__(256) void k_mask_map(const char * __restrict__ mask
 struct FwPlan { bool wide; int rows, nsplit, n_tiles, n_tb; size_t part, map; };
 constexpr size_t FW_JOIN_ROWS = 2048;   // from so many rows (times chunks) on the join takes a wave each: 4096 and four splits
                                         // 35 against 40 us in all, 1024 and sixteen 30 against 27
-constexpr int FW_MAP_TOK = 17;   // from so many tokens on the tile map is built by a launch of its own
+// From so many tokens of a workgroup on the tile map is built by a launch of its own, where a split has more than two tiles
+// (expanded, 16 heads, 16 tokens on 8192: 25 us with the map, 30 listing from the mask's rows; 32 on 4096: 22 and 36). Fewer
+// tokens are listed by every wave for itself (latent, 32 heads, 128 tokens on 1024 at 4 bits: 47.5, with the map 49.6), two
+// tiles are not listed at all (expanded, 20 tokens on 2048: 13.8, with the map 16.1)
+constexpr int FW_MAP_TOK = 5;
 
 // Rows of a workgroup and splits: those that end soonest by the times below, measured (us). A tile of a workgroup takes
 // t1 alone on its CU, t2 beside another (the absorbed form's tiles fill the LDS); its begin and end 6, the join 4 and
@@ -1270,7 +1274,7 @@ static FwPlan fw_plan(const ggml_tensor * dst) {
     }
     p.part = p.nsplit > 1 ? (size_t) p.nsplit * rows : 0;
     p.n_tb = (int) mx_ceil_div(q->ne[1], FW_TB);
-    if (m && m->ne[2] == 1 && q->ne[1] >= FW_MAP_TOK && p.n_tiles > 2) p.map = (size_t) m->ne[3] * p.n_tb * p.n_tiles;
+    if (m && m->ne[2] == 1 && std::min<int64_t>(q->ne[1], (p.rows + G - 2) / G + 1) >= FW_MAP_TOK && mx_ceil_div(p.n_tiles, p.nsplit) > 2) p.map = (size_t) m->ne[3] * p.n_tb * p.n_tiles;
     return p;
 }
 

@@ -427,6 +427,38 @@ def test_expanded_attention(ctx, backend, heads, kv_heads, n, m, S):
     assert rel(c.run(backend), c.want()) < ATT_REL
 
 
+def hidden_tiles(rng, S, H, n, m):
+    """causal; whole tiles hidden at random, the first ones from most tokens, and single keys"""
+    v = causal(S, n, m).copy()
+    tiles = -(-m // 32)
+    for t0 in range(0, n, 8):
+        for t in np.nonzero(rng.random(tiles) < 0.4)[0]:
+            v[:, :, t0:t0 + 8, 32 * t:32 * t + 32] = -np.inf
+    v[:, :, n // 3:, :70] = -np.inf
+    v[..., rng.random(m) < 0.02] = -np.inf
+    return v
+
+
+def window(rng, S, H, n, m):
+    """the last 150 keys of each token, and nothing for one of them"""
+    v = causal(S, n, m).copy()
+    for t in range(n):
+        v[:, :, t, :max(0, m - n + t - 150)] = -np.inf
+    v[-1, :, n // 2] = -np.inf
+    return v
+
+
+@pytest.mark.parametrize("mask", ["causal", hidden_tiles, window], ids=["causal", "hidden_tiles", "window"])
+@pytest.mark.parametrize("form,heads,n,m,S,cache", [("latent", 128, 80, 700, 1, "f16"), ("latent", 128, 30, 700, 2, "f16"), ("latent", 128, 62, 700, 1, "q8_0"),
+                                                    ("latent", 128, 31, 650, 2, "q4_0"), ("latent", 8, 1000, 1000, 1, "f16"), ("latent", 8, 700, 700, 1, "q4_0"),
+                                                    ("expanded", 64, 256, 600, 1, "f16"), ("expanded", 240, 20, 600, 1, "f16"), ("expanded", 128, 450, 450, 1, "f16")])
+def test_many_tiles_a_workgroup(ctx, backend, form, heads, n, m, S, cache, mask):
+    """enough rows that a workgroup walks 10 to 22 tiles: every slot of the rings several times, tiles listed from the mask's
+    rows and from the map, some left out, the ones fetched before the list among them"""
+    c = Case(ctx, form=form, heads=heads, n=n, m=m, S=S, cache=cache, mask=mask)
+    assert rel(c.run(backend), c.want()) < ATT_REL
+
+
 FORMS = [dict(form="latent", heads=8), dict(form="latent", heads=8, cache="q8_0"), dict(form="latent", heads=40), dict(form="latent", heads=40, cache="q4_0"),
          dict(form="expanded", heads=4), dict(form="expanded", heads=4, n=150, m=170),
          dict(form="latent", heads=128, n=70, m=110), dict(form="expanded", heads=512, n=66, m=80)]   # the variants of many rows
@@ -777,7 +809,7 @@ def test_graph_with_a_refused_node(pkg, ctx, backend):
 def test_kernel_choice(pkg, backend):
     """the rows of a workgroup go by the rows there are; more tokens than a few read the mask once for all heads"""
     for kw, want in ((dict(heads=16, n=1, m=600), "rows=32 "), (dict(heads=130, n=64, m=90), "rows=64 nsplit=1 "), (dict(heads=100, n=10, m=2000), "rows=64 nsplit=16"),
-                     (dict(heads=130, n=64, m=90, cache="q4_0"), "rows=32 "), (dict(heads=8, n=40, m=600), "map=1"),
+                     (dict(heads=130, n=64, m=90, cache="q4_0"), "rows=32 "), (dict(heads=8, n=200, m=1024), "map=1"), (dict(heads=32, n=40, m=600), "map=0"),
                      (dict(form="expanded", heads=2, n=1, m=600), "rows=32 "), (dict(form="expanded", heads=2, n=100, m=600), "rows=64 "),
                      (dict(form="expanded", heads=512, n=66, m=80), "rows=128 nsplit=1 ")):
         c = Case(pkg.Context(), **kw)
