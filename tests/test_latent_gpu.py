@@ -336,6 +336,24 @@ def test_append_outside_the_cache(ctx, backend):
     assert np.array_equal(out[rest], before[rest]) and not np.array_equal(out[2], before[2]) and not np.array_equal(out[7], before[7])
 
 
+@pytest.mark.parametrize("cache", ["f16", "f32"])
+def test_append_to_one_cell(ctx, backend, cache):
+    """several tokens of one cell: its values are theirs, each of one of them; the other cells are right"""
+    rng = np.random.default_rng(3)
+    n, n_ctx = 40, 16
+    g = latent_graph(ctx, n, n_ctx, cache, NEOX, True)
+    cells = np.full(n, 5, np.int64)
+    cells[:3] = [0, 9, 15]
+    x, w, pos = rng.standard_normal((n, 576)).astype(np.float32), np.ones(512, np.float32), np.arange(n, dtype=np.int32)
+    before = np.zeros((n_ctx, 576), np.float32 if cache == "f32" else np.float16)
+    out = run(ctx, backend, [g["out"]], [(g["x"], x), (g["w"], w), (g["pos"], pos), (g["idx"], cells), (g["cache"], before)])[0].reshape(n_ctx, 576)
+    want = latent_want(x, w, np.broadcast_to(pos, (4, n)), NEOX, True)[0]
+    off = np.abs(out[None, 5] - want[3:]).min(0)
+    half = EPS16 if cache == "f16" else 64 * EPS32
+    assert (off <= half * (1 + np.abs(want[3:]).max(0))).all()
+    assert np.abs(out[[0, 9, 15]] - want[:3]).max() <= half * (1 + np.abs(want[:3]).max()) and not out[[1, 2, 3, 4, 6, 7, 8]].any()
+
+
 # ---- attention whose keys are wider than its values -----------------------------------------------------
 def quantise(x, type_):
     """values -> cache bytes whose values (decode_rows) are the reference's"""
