@@ -727,10 +727,53 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
     fw_barrier();
 }
 
+// the last kind for f16: LDS-DMA, a wave eight rows of each piece; tile i + 2 beside tile i's scores
+template <int ROWS>
+__device__ __forceinline__ void fw_fetch(const FwArgs & p, const FwJob & j, char * ring) {
+    constexpr int BUF = 9 * FW_PIECE;
+    const int lane = threadIdx.x & 63, rowg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int srow = 8 * rowg + (lane >> 3), ssrc = 16 * ((lane & 7) ^ fw_swz(srow));
+    auto dma = [&](int tile, int slot) __attribute__((always_inline)) {
+        const int key0 = (tile & FW_TILE) * FW_KT, off = min(srow, p.n_kv - 1 - key0) * (int) p.k1 + ssrc;
+        const FwSrc src = fw_src(j.kb + (size_t) key0 * p.k1);
+        char * const to = ring + slot * BUF + 1024 * rowg;
+#pragma unroll
+        for (int i = 0; i < 9; ++i) fw_dma(src, off, 128 * i, to + i * FW_PIECE);
+    };
+    // the split's first two tiles on their way while the tiles are listed; as a rule they are the list's
+    const int s0 = j.tile(p, 0), s1 = j.tile(p, 1);
+    dma(s0, 0);
+    dma(s1, 1);
+    FwTiles tiles;
+    tiles.w0 = 0;
+    tiles.window<ROWS>(p, j);
+    int t0 = tiles.next<ROWS>(p, j), t1 = t0 >= 0 ? tiles.next<ROWS>(p, j) : -1, t2 = t1 >= 0 ? tiles.next<ROWS>(p, j) : -1;
+    if ((t0 >= 0 && (t0 & FW_TILE) != s0) || (t1 >= 0 && (t1 & FW_TILE) != s1)) {
+        fw_vmcnt<0>();                                          // (behind the ones under way to the same places)
+        dma(t0, 0);
+        dma(t1 >= 0 ? t1 : t0, 1);
+    }
+    fw_vmcnt<9>();
+    fw_barrier();
+    for (int slot = 2; t0 >= 0; slot = (slot + 1) & 3) {
+        if (t2 >= 0) dma(t2, slot);
+        fw_barrier();
+        if (t2 >= 0) fw_vmcnt<9>(); else fw_vmcnt<0>();         // the next tile has landed
+        t0 = t1;
+        t1 = t2;
+        if (t2 >= 0) t2 = tiles.next<ROWS>(p, j);
+        fw_barrier();
+    }
+    fw_vmcnt<0>();                                              // no DMA outlives the workgroup's LDS
+    fw_barrier();
+}
+
 template <int KV>
 __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
-    constexpr int NS = 9, ND = 16, ROWS = 32, AK = 2, AV = 2;   // fragments from LDS are read AK (AV) steps ahead
-    __shared__ __align__(128) char ring[3 * FQ_BUF];
+    constexpr bool QUANT = KV != GGML_TYPE_F16;
+    constexpr int NS = 9, ND = 16, ROWS = 32, AK = QUANT ? 2 : 3, AV = 2;      // fragments from LDS are read AK (AV) steps ahead
+    constexpr int RING = QUANT ? 3 : 4, BUF = QUANT ? FQ_BUF : 9 * FW_PIECE;
+    __shared__ __align__(128) char ring[RING * BUF];
     __shared__ __align__(16) wf4 exch[4][2][64];                // halves of scores
     __shared__ __align__(16) wf4 wgt[2][2][64];                 // weights: row group, 16 keys, the scores' lane
     __shared__ float scl[2][16];                                // a row's O takes this factor before them
@@ -742,7 +785,8 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
     const FwJob j = fw_job<ROWS, false>(p);
     if (wave >= 8) {
         __builtin_amdgcn_s_setprio(2);                          // (the longest of the three; without it 49 us instead of 47)
-        fw_produce<KV, ROWS>(p, j, ring, dtop);
+        if constexpr (QUANT) fw_produce<KV, ROWS>(p, j, ring, dtop);
+        else fw_fetch<ROWS>(p, j, ring);
         return;
     }
     const int r = min(j.r0 + 16 * rg + n16, j.nrow - 1);        // this lane's row
@@ -756,7 +800,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
         id0 = tiles.next<ROWS>(p, j);
         id1 = id0 >= 0 ? tiles.next<ROWS>(p, j) : -1;
         wh8 qh[NS], ql[NS];
-        const float qsc = fw_terms<NS>(p, qx, qh, ql) * (1.f / (1 << FQ_STEP));        // of this half's part of the scores
+        const float qsc = fw_terms<NS>(p, qx, qh, ql) * (QUANT ? 1.f / (1 << FQ_STEP) : 1.f);        // of this half's part of the scores
         const int kx0 = 128 * n16 + 16 * (g4 ^ fw_swz(n16)), kx1 = 128 * n16 + 16 * ((4 + g4) ^ fw_swz(n16));
         const int ka0 = dh ? kx1 + 4 * FW_PIECE : kx0, ka1 = dh ? kx0 + 5 * FW_PIECE : kx1;
         float m = -INFINITY, l = 0.f;
@@ -767,36 +811,45 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
         wf4 t[2];
         auto scores = [&](const char * buf) __attribute__((always_inline)) {
             wh8 a[AK + 1][2];
-            wh4 d[AK + 2][2];                                   // the blocks' steps of the lane's keys
-            wf4 x[2][2];
+            wh4 d[QUANT ? AK + 2 : 1][2];                       // the blocks' steps of the lane's keys
+            wf4 x[2][2];                                        // (f16: the low terms' products)
             auto lda = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     a[i % (AK + 1)][u] = *(const wh8 *) (buf + (i & 1 ? ka1 : ka0) + (i >> 1) * FW_PIECE + 2048 * u);
-                    d[i % (AK + 2)][u] = *(const wh4 *) (buf + 9 * FW_PIECE + 2 * ((NS * dh + i) * FW_KT + 16 * u + 4 * g4));
+                    if constexpr (QUANT) d[i % (AK + 2)][u] = *(const wh4 *) (buf + 9 * FW_PIECE + 2 * ((NS * dh + i) * FW_KT + 16 * u + 4 * g4));
                 }
             };
             auto step = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) t[u][c] = __builtin_fmaf((float) d[i % (AK + 2)][u][c], x[i & 1][u][c], t[u][c]);
+                    for (int c = 0; c < 4; ++c) t[u][c] = __builtin_fmaf((float) d[QUANT ? i % (AK + 2) : 0][u][c], x[i & 1][u][c], t[u][c]);
             };
             t[0] = t[1] = wf4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (!QUANT) x[0][0] = x[0][1] = t[0];
 #pragma unroll
             for (int i = 0; i < AK; ++i) lda(i);
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 if (i + AK < NS) lda(i + AK);
-                // one 32-block a step: its products are whole, then, a step later, take the block's step
+                if constexpr (!QUANT) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], wf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    for (int u = 0; u < 2; ++u) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], t[u], 0, 0, 0);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], x[i & 1][u], 0, 0, 0);
-                if (i) step(i - 1);
+                    for (int u = 0; u < 2; ++u) x[0][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], x[0][u], 0, 0, 0);
+                } else {
+                    // one 32-block a step: its products are whole, then, a step later, take the block's step
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], qh[i], wf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) x[i & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (AK + 1)][u], ql[i], x[i & 1][u], 0, 0, 0);
+                    if (i) step(i - 1);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            step(NS - 1);
+            if constexpr (QUANT) step(NS - 1);
+            else { t[0] += x[0][0]; t[1] += x[0][1]; }
             t[0] *= qsc;
             t[1] *= qsc;
             exch[wave][0][lane] = t[0];
@@ -805,23 +858,25 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
         // the scores whole, the reference maximum, this wave's 16 keys' weights
         auto softmax = [&](int tile, int slot) __attribute__((always_inline)) {
             wf4 s[2] = {t[0] + exch[wave ^ 1][0][lane], t[1] + exch[wave ^ 1][1][lane]};
-            float top = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, dtop[slot][i]);
             if (p.softcap != 0.0f) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = p.softcap * tanhf(s[i >> 2][i & 3]);
             }
             if (tile >> 30) fw_mask(p, j, r, tile & FW_TILE, s);
             float f = 1.f;
-            const int x = top < INFINITY ? __builtin_amdgcn_frexp_expf(top) + FQ_STEP : 0;
-            if (x > qe) {                                       // the same in every wave; on the first tiles only
-                f = __builtin_amdgcn_ldexpf(1.f, qe - x);
-                qe = x;
+            if constexpr (QUANT) {
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, dtop[slot][i]);
+                const int x = top < INFINITY ? __builtin_amdgcn_frexp_expf(top) + FQ_STEP : 0;
+                if (x > qe) {                                   // the same in every wave; on the first tiles only
+                    f = __builtin_amdgcn_ldexpf(1.f, qe - x);
+                    qe = x;
+                }
             }
             wf4 one[1] = {wf4{f, 0.f, 0.f, 0.f}};               // O's factor
             const float ms = fw_raise<1>(s, m, l, one);
-            const float qf = __builtin_amdgcn_ldexpf(1.f, 7 - qe);
+            const float qf = QUANT ? __builtin_amdgcn_ldexpf(1.f, 7 - qe) : 1.f;
             const wf4 sv = dh ? s[1] : s[0];
             wf4 e;
 #pragma unroll
@@ -833,8 +888,8 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
             if (dh == 0 && g4 == 0) scl[rg][n16] = one[0][0];
         };
         fw_barrier();
-        for (int slot = 0; id0 >= 0; slot = slot == 2 ? 0 : slot + 1) {
-            scores(ring + slot * FQ_BUF);
+        for (int slot = 0; id0 >= 0; slot = slot == RING - 1 ? 0 : slot + 1) {
+            scores(ring + slot * BUF);
             fw_barrier();
             softmax(id0, slot);
             id0 = id1;
@@ -858,13 +913,13 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) va[i] = (4 * dh + p.vpiece) * FW_PIECE + 128 * vrow + 16 * ((2 * i + (ip >> 1)) ^ vsw) + 8 * (ip & 1);
     const int vstep = 9 * FW_PIECE + 2 * ((8 * dh + 2 * p.vpiece) * FW_KT + 4 * g4);
-    wh8 v[AV + 1][2], ph[2], pl[2];                             // (terms of a block's weights, and of the next one's)
-    wh4 vd[AV + 1][2];
+    wh8 v[AV + 1][2], ph[QUANT ? 2 : 1], pl[QUANT ? 2 : 1];     // (quantised: terms of a block's weights, and of the next one's)
+    wh4 vd[QUANT ? AV + 1 : 1][2];
     float e[8];
     wh2 eh[4];
     auto ldv = [&](const char * buf, int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) vd[b % (AV + 1)][u] = *(const wh4 *) (buf + vstep + 2 * (b * FW_KT + 16 * u));
+        for (int u = 0; u < 2; ++u) if constexpr (QUANT) vd[b % (AV + 1)][u] = *(const wh4 *) (buf + vstep + 2 * (b * FW_KT + 16 * u));
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const char * a_ = buf + va[2 * (b & 1) + c] + (b >> 1) * FW_PIECE;
@@ -880,8 +935,8 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
     auto terms = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-            const wh4 d = vd[b % (AV + 1)][i >> 2];
-            split2p(e[i], e[i + 1], eh[i >> 1], wh2{d[i & 3], d[(i & 3) + 1]}, i, ph[b & 1], pl[b & 1]);
+            const wh4 d = vd[QUANT ? b % (AV + 1) : 0][i >> 2];
+            split2p(e[i], e[i + 1], eh[i >> 1], wh2{d[i & 3], d[(i & 3) + 1]}, i, ph[QUANT ? b & 1 : 0], pl[QUANT ? b & 1 : 0]);
         }
     };
     // O^T += V^T P^T, 32-blocks b0 .. b1 - 1 of this wave's channels
@@ -889,8 +944,8 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
 #pragma unroll
         for (int b = b0; b < b1; ++b) {
             if (b + AV < ND / 2) ldv(buf, b + AV);
-            if (b + 1 < ND / 2) terms(b + 1);
-            const int w = b & 1;
+            if constexpr (QUANT) { if (b + 1 < ND / 2) terms(b + 1); }
+            const int w = QUANT ? b & 1 : 0;
             o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], ph[w], o[2 * b], 0, 0, 0);
             o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][1], ph[w], o[2 * b + 1], 0, 0, 0);
             o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b % (AV + 1)][0], pl[w], o[2 * b], 0, 0, 0);
@@ -909,7 +964,8 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= f;
         }
-        terms(0);
+        if constexpr (QUANT) terms(0);
+        else split8(e, ph[0], pl[0]);
     };
     fw_barrier();
     if (id0 >= 0) {
@@ -917,22 +973,24 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
         ahead(ring);
         fw_barrier();
         for (int slot = 0;;) {                                  // the tile in `slot`; beside it the next one's scores
-            const char * buf = ring + slot * FQ_BUF;
+            const char * buf = ring + slot * BUF;
             weights();
             values(buf, 0, ND / 4);
             if (id1 >= 0) fw_barrier();
             values(buf, ND / 4, ND / 2);
             if (id1 < 0) break;
             id1 = tiles.next<ROWS>(p, j);
-            slot = slot == 2 ? 0 : slot + 1;
-            ahead(ring + slot * FQ_BUF);
+            slot = slot == RING - 1 ? 0 : slot + 1;
+            ahead(ring + slot * BUF);
             fw_barrier();
         }
     }
     fw_barrier();
-    const float f = __builtin_amdgcn_ldexpf(1.f, endq - 7 - FQ_STEP);
+    if constexpr (QUANT) {
+        const float f = __builtin_amdgcn_ldexpf(1.f, endq - 7 - FQ_STEP);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) o[d] *= f;
+        for (int d = 0; d < ND; ++d) o[d] *= f;
+    }
     fw_store<576, 512, KV, ND>(p, j, j.kb, p.k1, 64 * p.vpiece, j.r0 + 16 * rg, 256 * dh, endm[rg][lane], endl[rg][0][lane] + endl[rg][1][lane], o);
 }
 
@@ -1360,7 +1418,7 @@ void fa_wide_run(OpCtx & c, ggml_tensor * dst) {
         else        k_fattn_expanded<2, 4><<<grid, 256, 0, c.st>>>(a);
     } else if (k->type == GGML_TYPE_Q8_0) k_fattn_latent_q<GGML_TYPE_Q8_0><<<grid, 768, 0, c.st>>>(a);
     else if (k->type == GGML_TYPE_Q4_0) k_fattn_latent_q<GGML_TYPE_Q4_0><<<grid, 768, 0, c.st>>>(a);
-    else if (pl.rows == 32) k_fattn_latent<2><<<grid, FlGeo<2>::NT, 0, c.st>>>(a);
+    else if (pl.rows == 32) k_fattn_latent_q<GGML_TYPE_F16><<<grid, 768, 0, c.st>>>(a);
     else k_fattn_latent<4><<<grid, FlGeo<4>::NT, 0, c.st>>>(a);
     if (pl.nsplit > 1) {
         const unsigned rows = (unsigned) (a.S * a.n_q * a.H), chunks = (unsigned) (DV / std::min(DV, 256));
