@@ -392,31 +392,19 @@ __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, cons
 }
 
 // ---- absorbed: K rows of 576, V in them --------------------------------------------------------------
-// RG groups of 16 rows, two waves each. O of 16 rows is 128 registers a lane and Q (two terms) 144, too
+// Many rows, f16: four groups of 16, two waves each. O of 16 rows is 128 registers a lane and Q (two terms) 144, too
 // much for one wave beside the rest of it, so the pair shares: wave dh multiplies channels [288 dh, + 288)
 // of the keys, the halves of the scores are exchanged through LDS (the only barrier of a tile), both do
 // the softmax, and each keeps half of the output channels.
-// Few rows (RG = 2): the cache bounds it. 4 sequences of up to 32768 tokens, 32 heads: 38 us for 123.5 MB, 6 TB/s while it
-// streams (a large copy 5.2), 4 us before and 2 behind, the join 5.4. Many (RG = 4): the matrix unit and its power. 512
-// tokens, 32 heads, 4096 keys: 250 us warm, 1.08 PFLOP/s of f16 products (a large library product 1.18); a build of
-// 14 % fewer busy cycles took the same time at a clock lower by as much
-template <int RG> struct FlGeo {
-    static constexpr int NT = 128 * RG;                         // threads
-    // tiles in the ring, three ahead of the one in use where they fit beside the exchange
-    static constexpr int RING = RG == 2 ? 4 : 3;
-    static constexpr int BUF = 9 * FW_PIECE;
-    static constexpr int DMA = (36 + 2 * RG - 1) / (2 * RG);    // LDS-DMA instructions of a wave and tile
-};
-
-template <int RG>
-__global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
-    using geo = FlGeo<RG>;
-    constexpr int RING = geo::RING, NS = 9, ND = 16, ROWS = 16 * RG, NW = 2 * RG;
+// The matrix unit and its power bound it. 512 tokens, 32 heads, 4096 keys: 250 us warm, 1.08 PFLOP/s of f16 products (a
+// large library product 1.18); a build of 14 % fewer busy cycles took the same time at a clock lower by as much. The form
+// of 32 rows below takes 278
+__global__ __launch_bounds__(512, 2) void k_fattn_latent64(FwArgs p) {
+    constexpr int NS = 9, ND = 16, ROWS = 64, NW = 8, BUF = 9 * FW_PIECE, DMA = 5;         // LDS-DMA instructions of a wave and tile
     // the ring's tiles as objects of their own: reads of one need not wait for the DMA that fills another
-    __shared__ __align__(128) char t0[geo::BUF];
-    __shared__ __align__(128) char t1[geo::BUF];
-    __shared__ __align__(128) char t2[geo::BUF];
-    __shared__ __align__(128) char t3[RING == 4 ? geo::BUF : 16];
+    __shared__ __align__(128) char t0[BUF];
+    __shared__ __align__(128) char t1[BUF];
+    __shared__ __align__(128) char t2[BUF];
     __shared__ __align__(16) wf4 exch[2][NW][2][64];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -432,38 +420,38 @@ __global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
     const int srow = 8 * (wave & 3) + (lane >> 3), ssrc = 16 * ((lane & 7) ^ fw_swz(srow));
     auto dma_off = [&](int tile) { return min(srow, p.n_kv - 1 - (tile & FW_TILE) * FW_KT) * (int) p.k1 + ssrc; };
     auto dma_src = [&](int tile) { return fw_src(j.kb + (size_t) ((tile & FW_TILE) * FW_KT) * p.k1); };
-    // instruction i of a wave: it keeps to one row group (wave & 3); of eight waves, two share one and halve its pieces
+    // instruction i of a wave: it keeps to one row group (wave & 3); two waves share one and halve its pieces
     auto dma = [&](const FwSrc & src, int off, char * buf, int i) __attribute__((always_inline)) {
-        const int piece = NW == 8 ? min(2 * i + (wave >> 2), 8) : i;        // (piece 8 is brought twice)
+        const int piece = min(2 * i + (wave >> 2), 8);          // (piece 8 is brought twice)
         fw_dma(src, off, 128 * piece, buf + piece * FW_PIECE + 1024 * (wave & 3));
     };
     // ---- the split's first tiles on their way while the tiles are listed; as a rule they are the list's.
     // id[c]: the tile in slot c of the ring (-1: none)
-    char * const ring[4] = {t0, t1, t2, t3};
-    int id[RING];
+    char * const ring[3] = {t0, t1, t2};
+    int id[3];
     auto dma_tile = [&](int tile, char * buf) __attribute__((always_inline)) {
         const FwSrc src = dma_src(tile);
         const int off = dma_off(tile);
 #pragma unroll
-        for (int i = 0; i < geo::DMA; ++i) dma(src, off, buf, i);
+        for (int i = 0; i < DMA; ++i) dma(src, off, buf, i);
     };
 #pragma unroll
-    for (int c = 0; c < RING - 1; ++c) if (c < j.nl) dma_tile(j.tile(p, c), ring[c]);
+    for (int c = 0; c < 2; ++c) if (c < j.nl) dma_tile(j.tile(p, c), ring[c]);
     FwTiles tiles;
     tiles.w0 = 0;
     tiles.window<ROWS>(p, j);
     bool listed = true;
 #pragma unroll
-    for (int c = 0; c < RING - 1; ++c) {
+    for (int c = 0; c < 2; ++c) {
         id[c] = c == 0 || id[c - 1] >= 0 ? tiles.next<ROWS>(p, j) : -1;
         listed &= id[c] < 0 || (id[c] & FW_TILE) == j.tile(p, c);
     }
     if (!listed) {
         fw_vmcnt<0>();                                          // (behind the ones under way to the same places)
 #pragma unroll
-        for (int c = 0; c < RING - 1; ++c) if (id[c] >= 0) dma_tile(id[c], ring[c]);
+        for (int c = 0; c < 2; ++c) if (id[c] >= 0) dma_tile(id[c], ring[c]);
     }
-    id[RING - 1] = id[RING - 2] >= 0 ? tiles.next<ROWS>(p, j) : -1;         // fetched by the first body
+    id[2] = id[1] >= 0 ? tiles.next<ROWS>(p, j) : -1;           // fetched by the first body
     wh8 qh[NS], ql[NS];
     const float qsc = fw_terms<NS>(p, qx, qh, ql);              // of this half's part of the scores
 
@@ -514,7 +502,7 @@ __global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
         wf4 tl[2] = {t[0], t[0]};                               // a chain of its own for the low term
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            if constexpr (W) { if (i < geo::DMA) dma(fsrc, foff, fbuf, i); }
+            if constexpr (W) { if (i < DMA) dma(fsrc, foff, fbuf, i); }
             if (i + AK < NS) lda(buf, i + AK);
             if (W && i >= NS - AV) ldv(vbuf, i - (NS - AV));
 #pragma unroll
@@ -535,9 +523,9 @@ __global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
         exch[par][wave][0][lane] = t[0];
         exch[par][wave][1][lane] = t[1];
     };
-    // behind the barrier: the scores of tile `tile` (slot C) whole, the reference maximum; the first fragments of the
+    // behind the barrier: the scores of tile `tile` whole, the reference maximum; the first fragments of the
     // tile in `buf` meanwhile
-    auto whole = [&](int tile, const int C, const char * buf) __attribute__((always_inline)) {
+    auto whole = [&](int tile, const char * buf) __attribute__((always_inline)) {
         const wf4 x0 = exch[par][wave ^ 1][0][lane], x1 = exch[par][wave ^ 1][1][lane];
         __builtin_amdgcn_sched_barrier(0);
         ahead(buf);
@@ -568,14 +556,14 @@ __global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
     // matrix instructions of the next tile's scores, the exchange passes under this tile's values. The barrier then
     // frees slot C (and tells that the tile after the next is whole)
     auto body = [&](auto slot_) __attribute__((always_inline)) {
-        constexpr int C = decltype(slot_)::value, C1 = (C + 1) % RING, F = (C + RING - 1) % RING;
+        constexpr int C = decltype(slot_)::value, C1 = (C + 1) % 3, F = (C + 2) % 3;
         const int further = id[F] >= 0 ? id[F] : id[C];         // (behind the last tile: any, into a place no longer read)
         scores(ring[C1], ring[C], ring[F], dma_src(further), dma_off(further), std::true_type{});
         values(ring[C]);
-        fw_vmcnt<(RING - 3) * geo::DMA>();                      // the tile after the next has landed
+        fw_vmcnt<0>();                                          // the tile after the next has landed
         fw_barrier();
         id[C] = id[F] >= 0 ? tiles.next<ROWS>(p, j) : -1;
-        whole(id[C1], C1, ring[(C + 2) % RING]);                // (fragments read for nothing where no such tile is left)
+        whole(id[C1], ring[F]);                                 // (fragments read for nothing where no such tile is left)
     };
 
     fw_vmcnt<0>();
@@ -584,7 +572,7 @@ __global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
         ahead(t0);
         scores(t0, t0, nullptr, dma_src(id[0]), 0, std::false_type{});
         fw_barrier();
-        whole(id[0], 0, t1);
+        whole(id[0], t1);
         const char * last;
         for (;;) {
             last = t0;
@@ -594,13 +582,8 @@ __global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
             if (id[2] < 0) break;
             body(std::integral_constant<int, 1>{});
             last = t2;
-            if (id[3 % RING] < 0) break;
+            if (id[0] < 0) break;
             body(std::integral_constant<int, 2>{});
-            if constexpr (RING == 4) {
-                last = t3;
-                if (id[0] < 0) break;
-                body(std::integral_constant<int, 3>{});
-            }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -616,20 +599,25 @@ __global__ __launch_bounds__(128 * RG, RG / 2) void k_fattn_latent(FwArgs p) {
     fw_store<576, 512, GGML_TYPE_F16, ND>(p, j, j.kb, p.k1, 64 * p.vpiece, j.r0 + 16 * rg, 256 * dh, m, l, o);
 }
 
-// ---- absorbed, quantised ------------------------------------------------------------------------------
+// ---- absorbed, few rows, and quantised -----------------------------------------------------------------
 // 32 rows, and the work of a tile dealt out by kind, one wave of each kind a SIMD, so that one's waits are filled by the
-// others' vector instructions (they bound it: a block's step enters its products, and V's steps the weights, in 32 bits):
+// others' instructions:
 //   4 waves   scores of the next tile (a pair of waves a row group, as above), its softmax; the weights go through LDS
 //   4 waves   values of this tile, half of the channels of a row group each
-//   4 waves   blocks of the tile after the next into f16 integers
-// Two barriers a tile: behind the halves of the scores, and behind the weights. A tile on every CU at once, 4 bits: 2.6 us
-// with all of it in one wave a SIMD, 2.2 with the last kind apart, 1.9 so; alone on the chip 2.6, 1.8 and 1.5 (8 bits 1.65).
-// 4 x 32768 tokens at 4 bits: 40 us for 34.7 MB, 250 before the kinds were parted and the steps read ahead. What is left is
-// the chain of one tile: 500 vector instructions and 68 matrix instructions a SIMD, 2000 and 1100 of some 3800 cycles
+//   4 waves   the tile after the next: f16 fetched by LDS-DMA into a ring of four (all 160 KB, with what is exchanged);
+//             quantised, blocks turned into f16 integers, a ring of three
+// Two barriers a tile: behind the halves of the scores, and behind the weights.
+// f16: the cache bounds it. 4 sequences of up to 32768 tokens, 32 heads: 33 us for 123.5 MB (a large copy takes 24), the
+// join 5.4 more; one wave doing scores and values in turn took 38, and alone on the chip 1.33 us a
+// tile instead of 1.0. 200 tokens on 512 keys 26.9 us, 32.2 then.
+// Quantised, a tile on every CU at once, 4 bits: 2.6 us with all of it in one wave a SIMD, 2.2 with the last kind apart, 1.9
+// so; alone on the chip 2.6, 1.8 and 1.5 (8 bits 1.65). 4 x 32768 tokens at 4 bits: 39 us for 34.7 MB. What is left is the
+// chain of one tile and the vector unit (a block's step enters its products, and V's steps the weights, in 32 bits): 500
+// vector instructions and 68 matrix instructions a SIMD, 2000 and 1100 of some 3800 cycles
 constexpr int FQ_BUF = 9 * FW_PIECE + 18 * FW_KT * 2;           // a tile and its blocks' steps, [block][key] f16, ...
 constexpr int FQ_STEP = 10;                                     // ... times 2^10, out of the range where f16 keeps few bits
 
-// the last kind: blocks through registers, two tiles ahead of the store
+// the last kind, quantised: blocks through registers, two tiles ahead of the store
 template <int KV, int ROWS>
 __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, char * ring, float (&dtop)[3][4]) {
     // eight threads a row take two whole 32-blocks each, x and x + 8, and eight values of the last two blocks. A block
@@ -769,7 +757,7 @@ __device__ __forceinline__ void fw_fetch(const FwArgs & p, const FwJob & j, char
 }
 
 template <int KV>
-__global__ __launch_bounds__(768, 3) void k_fattn_latent_q(FwArgs p) {
+__global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
     constexpr bool QUANT = KV != GGML_TYPE_F16;
     constexpr int NS = 9, ND = 16, ROWS = 32, AK = QUANT ? 2 : 3, AV = 2;      // fragments from LDS are read AK (AV) steps ahead
     constexpr int RING = QUANT ? 3 : 4, BUF = QUANT ? FQ_BUF : 9 * FW_PIECE;
@@ -1304,14 +1292,14 @@ constexpr int FW_MAP_TOK = 5;
 
 // Rows of a workgroup and splits: those that end soonest by the times below, measured (us). A tile of a workgroup takes
 // t1 alone on its CU, t2 beside another (the absorbed form's tiles fill the LDS); its begin and end 6, the join 4 and
-// 1 for 8 MB of partial results. Absorbed, f16, 32 heads: 64 tokens, 1024 keys 35 with 32 rows and 4 splits (64 rows, 8
-// splits: 37); 512 tokens 285 with 64 rows (32: more than 400)
+// 1 for 8 MB of partial results. Absorbed, f16, 32 heads: 64 tokens, 1024 keys 29.6 with 32 rows and 4 splits (64 rows, 8
+// splits: 35); 512 tokens, 4096 keys 257 with 64 rows (32: 278)
 // Expanded: 128 rows where they fill every CU twice (2048 tokens and keys, 32 heads: 118 against 134 with 64), else 64
 // (499 tokens: 26 against 39); 32 for no more rows than that (16 tokens, 1024 keys 14.6 against 15.8)
 struct FwRows { int rows; double t1, t2; };
 static FwPlan fw_plan(const ggml_tensor * dst) {
     const ggml_tensor * q = dst->src[0], * k = dst->src[1], * v = dst->src[2], * m = dst->src[3];
-    static const FwRows latent[2] = {{32, 1.33, 0}, {64, 1.63, 0}}, quant[1] = {{32, 1.55, 0}}, expanded[3] = {{32, 1.03, 1.27}, {64, 0.93, 1.46}, {128, 1.45, 2.8}};
+    static const FwRows latent[2] = {{32, 1.0, 0}, {64, 1.63, 0}}, quant[1] = {{32, 1.55, 0}}, expanded[3] = {{32, 1.03, 1.27}, {64, 0.93, 1.46}, {128, 1.45, 2.8}};
     FwPlan p{};
     p.wide = k->ne[0] == 576;
     const int64_t G = q->ne[2] / k->ne[2], nrow = q->ne[1] * G, units = k->ne[2] * q->ne[3];
@@ -1416,10 +1404,10 @@ void fa_wide_run(OpCtx & c, ggml_tensor * dst) {
         if (pl.rows == 32) k_fattn_expanded<1, 2><<<grid, 128, 0, c.st>>>(a);
         else if (pl.rows == 64) k_fattn_expanded<1, 4><<<grid, 256, 0, c.st>>>(a);
         else        k_fattn_expanded<2, 4><<<grid, 256, 0, c.st>>>(a);
-    } else if (k->type == GGML_TYPE_Q8_0) k_fattn_latent_q<GGML_TYPE_Q8_0><<<grid, 768, 0, c.st>>>(a);
-    else if (k->type == GGML_TYPE_Q4_0) k_fattn_latent_q<GGML_TYPE_Q4_0><<<grid, 768, 0, c.st>>>(a);
-    else if (pl.rows == 32) k_fattn_latent_q<GGML_TYPE_F16><<<grid, 768, 0, c.st>>>(a);
-    else k_fattn_latent<4><<<grid, FlGeo<4>::NT, 0, c.st>>>(a);
+    } else if (k->type == GGML_TYPE_Q8_0) k_fattn_latent32<GGML_TYPE_Q8_0><<<grid, 768, 0, c.st>>>(a);
+    else if (k->type == GGML_TYPE_Q4_0) k_fattn_latent32<GGML_TYPE_Q4_0><<<grid, 768, 0, c.st>>>(a);
+    else if (pl.rows == 32) k_fattn_latent32<GGML_TYPE_F16><<<grid, 768, 0, c.st>>>(a);
+    else k_fattn_latent64<<<grid, 512, 0, c.st>>>(a);
     if (pl.nsplit > 1) {
         const unsigned rows = (unsigned) (a.S * a.n_q * a.H), chunks = (unsigned) (DV / std::min(DV, 256));
         if (rows * (size_t) chunks >= FW_JOIN_ROWS) {

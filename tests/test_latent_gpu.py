@@ -425,7 +425,7 @@ class Case:
 
 LATENT_SHAPES = [  # heads, n, m, S
     (4, 1, 1, 1), (16, 1, 63, 1), (32, 1, 64, 1), (32, 1, 65, 1), (10, 3, 300, 1), (32, 1, 1000, 3), (64, 1, 129, 2), (128, 1, 200, 1), (1, 1, 700, 1),
-    (40, 17, 150, 1), (8, 33, 200, 2), (4, 100, 100, 1), (16, 40, 640, 1), (1, 70, 70, 1), (130, 64, 90, 1), (100, 10, 2000, 1),
+    (40, 17, 150, 1), (8, 33, 200, 2), (4, 100, 100, 1), (16, 40, 640, 1), (1, 70, 70, 1), (130, 64, 90, 1), (100, 10, 2000, 1), (128, 40, 1200, 1),
 ]
 
 
@@ -826,7 +826,7 @@ def test_graph_with_a_refused_node(pkg, ctx, backend):
 
 def test_kernel_choice(pkg, backend):
     """the rows of a workgroup go by the rows there are; more tokens than a few read the mask once for all heads"""
-    for kw, want in ((dict(heads=16, n=1, m=600), "rows=32 "), (dict(heads=130, n=64, m=90), "rows=64 nsplit=1 "), (dict(heads=100, n=10, m=2000), "rows=64 nsplit=16"),
+    for kw, want in ((dict(heads=16, n=1, m=600), "rows=32 "), (dict(heads=130, n=64, m=90), "rows=64 nsplit=1 "), (dict(heads=128, n=40, m=1200), "rows=64 nsplit=3 "),
                      (dict(heads=130, n=64, m=90, cache="q4_0"), "rows=32 "), (dict(heads=8, n=200, m=1024), "map=1"), (dict(heads=32, n=40, m=600), "map=0"),
                      (dict(form="expanded", heads=2, n=1, m=600), "rows=32 "), (dict(form="expanded", heads=2, n=100, m=600), "rows=64 "),
                      (dict(form="expanded", heads=512, n=66, m=80), "rows=128 nsplit=1 ")):
