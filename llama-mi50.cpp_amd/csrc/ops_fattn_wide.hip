@@ -342,7 +342,10 @@ __device__ __forceinline__ void fw_again(const FwArgs & p, const FwJob & j, cons
 }
 
 // The end of a row group of 16: the lanes' sums joined, rows with a NaN computed again, the result (or
-// the split's part of it) stored. o[d]: channels d0 + 16 d + 4 g4 + 0..3 of row r; D0: d0 == 0 stores m, l
+// the split's part of it) stored. o[d]: channels d0 + 16 d + 4 g4 + 0..3 of row r; D0: d0 == 0 stores m, l.
+// Where two waves hold a row's channels, one of them may have to compute its half again and the other not. Both have the same
+// m and l, so the half takes m as its reference (the sums of fw_again are relative to the keys' own maximum, other by up to
+// what fw_raise lets pass), and both take the new m and l only where l itself is no number
 template <int DK, int DV, int KV, int ND>
 __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, const char * vb, size_t v1, int vd0, int rg0, int d0, float m, float l, wf4 (&o)[ND]) {
     const int lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
@@ -357,14 +360,15 @@ __device__ __forceinline__ void fw_store(const FwArgs & p, const FwJob & j, cons
         const int col = __builtin_ctz(bad);
         float m2, l2, acc[ND / 4];
         fw_again<DK, KV, ND / 4>(p, j, vb, v1, min(rg0 + col, j.nrow - 1), vd0 + d0, m2, l2, acc);
+        if (n16 == col && l * 0.f != 0.f) { m = m2; l = l2; }
+        const float f = m2 == m ? 1.f : __builtin_amdgcn_exp2f(m2 - m);     // (of the lanes of that row)
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float v = __shfl(acc[d >> 2], 16 * (d & 3) + 4 * g4 + i, 64);
-                if (n16 == col) o[d][i] = v;
+                if (n16 == col) o[d][i] = v * f;
             }
-        if (n16 == col) { m = m2; l = l2; }
     }
     const int r = rg0 + n16;
     if (r >= j.nrow) return;
