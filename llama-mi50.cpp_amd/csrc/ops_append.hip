@@ -456,7 +456,7 @@ int fuse_append_rows(OpCtx & c, ggml_cgraph * g, int i, const UseCount & use_map
         keep_mul = !single(mul, ms);
         const int64_t d = nx->ne[0];
         if (nx->type != GGML_TYPE_F32 || norm->type != GGML_TYPE_F32 || mul->type != GGML_TYPE_F32 || nx->nb[0] != 4 || mx_nrows(nx) != ntok ||
-            !mx_are_same_shape(mul, norm) || w->type != GGML_TYPE_F32 || mx_nelements(w) != d || w->nb[0] != 4 || d > APPEND_MAX_ROW) return 0;
+            !mx_are_same_shape(mul, norm) || w->type != GGML_TYPE_F32 || w->ne[0] != d || mx_nelements(w) != d || w->nb[0] != 4 || d > APPEND_MAX_ROW) return 0;
         // tokens along dimension 1 or 2 of the norm's input, rows of one head
         if (!((nx->ne[1] == ntok && nx->ne[2] == 1) || (nx->ne[1] == 1 && nx->ne[2] == ntok)) || nx->ne[3] != 1) return 0;
         if (cat->ne[0] != d + turned || cat->ne[1] != 1 || ms->ne[0] != d || rs->ne[0] != p.dim || p.heads != 1 || p.k.width != d + turned) return 0;
