@@ -9,7 +9,8 @@
 //
 // Precision: the result is f32 and callers ask for GGML_PREC_F32, so nothing is rounded to 11 bits on
 // the way: q (scaled by a power of two into f16's range) and the softmax weights enter the f16 matrix
-// units as two terms, high + low (22 bits), each product twice; K and V are exact in f16, quantised
+// units as two terms, high + low, each product twice: 22 bits, for a weight down to 2^-10 of the row's largest, below
+// that 2^-32 of the largest; K and V are exact in f16, quantised
 // ones as their integers: a block's step is applied in f32 to the products of K, and to the weights of V
 // as their terms are formed. The rate that bounds the large cases is therefore half the f16 rate.
 //
@@ -61,17 +62,24 @@ struct FwArgs {
 
 __device__ __forceinline__ uint4 ldu16(const char * p) { uint4 v; __builtin_memcpy(&v, p, 16); return v; }
 
-// hi + lo = x to 22 bits: the high term truncated, the remainder (exact in f32) truncated again
+// two values to f16, to nearest: what many small weights leave out then has either sign (cut off, 4096 weights of 2^-17 of
+// the largest take 2e-5 from the result, 32768 of 2^-20 1e-4)
+__device__ __forceinline__ wh2 fw_near(float x0, float x1) {
+    typedef float wf2 __attribute__((ext_vector_type(2)));
+    return __builtin_convertvector((wf2{x0, x1}), wh2);
+}
+// hi + lo = x to 22 bits, or to 2^-25 where x is below 2^-3 (f16's smallest step is 2^-24): the high term truncated, the
+// remainder (exact in f32) rounded
 __device__ __forceinline__ void split2(float x0, float x1, int j, wh8 & hi, wh8 & lo) {
     const wh2 h = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-    const wh2 l = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(x0 - (float) h[0], x1 - (float) h[1]));
+    const wh2 l = fw_near(x0 - (float) h[0], x1 - (float) h[1]);
     hi[j] = h[0]; hi[j + 1] = h[1];
     lo[j] = l[0]; lo[j + 1] = l[1];
 }
 // the same of the products x0 d0, x1 d1, h being x0 and x1 to f16: the high terms multiplied there, the remainder of the whole product
 __device__ __forceinline__ void split2p(float x0, float x1, wh2 h, wh2 d, int j, wh8 & hi, wh8 & lo) {
     h *= d;
-    const wh2 l = __builtin_bit_cast(wh2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(x0, (float) d[0], -(float) h[0]), __builtin_fmaf(x1, (float) d[1], -(float) h[1])));
+    const wh2 l = fw_near(__builtin_fmaf(x0, (float) d[0], -(float) h[0]), __builtin_fmaf(x1, (float) d[1], -(float) h[1]));
     hi[j] = h[0]; hi[j + 1] = h[1];
     lo[j] = l[0]; lo[j + 1] = l[1];
 }
@@ -272,14 +280,17 @@ __device__ __forceinline__ void fw_mask(const FwArgs & p, const FwJob & j, int r
 }
 
 // Online softmax of a lane's row over its 8 keys of the tile and the other three lanes' (the row lies in
-// four). First the reference maximum: raised only when a score exceeds it by 8 (weights up to 2^8), so
-// O is rescaled on the first tiles only. Returns -m for the weights 2^(s - m).
+// four). First the reference: FW_LOW below the maximum that it was taken from, so weights use f16's whole range and a small
+// one keeps its bits down to 2^-32 of the largest; raised only when a score exceeds that maximum by 8 (weights up to
+// 2^15), so O is rescaled on the first tiles only. Returns -m for the weights 2^(s - m).
+constexpr float FW_LOW = 7.f;
 template <int ND>
 __device__ __forceinline__ float fw_raise(const wf4 (&s)[2], float & m, float & l, wf4 (&o)[ND]) {
     float mt = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     mt = fw_row4<false>(mt);
-    const bool raise = mt > m + 8.f;                            // false while nothing was visible
+    const bool raise = mt > m + (FW_LOW + 8.f);                 // false while nothing was visible
     if (__any(raise)) {
+        mt -= FW_LOW;
         const float al = raise ? __builtin_amdgcn_exp2f(m - mt) : 1.f;
         if (raise) m = mt;
         l *= al;
@@ -796,8 +807,8 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
         const int kx0 = 128 * n16 + 16 * (g4 ^ fw_swz(n16)), kx1 = 128 * n16 + 16 * ((4 + g4) ^ fw_swz(n16));
         const int ka0 = dh ? kx1 + 4 * FW_PIECE : kx0, ka1 = dh ? kx0 + 5 * FW_PIECE : kx1;
         float m = -INFINITY, l = 0.f;
-        // the weights take V's steps before they are split, so they and O are held in units of 2^(qe - 7), 2^qe the
-        // largest (scaled) step seen, 1 at least: weights, up to 2^8, and their products with steps stay in f16's range.
+        // the weights take V's steps before they are split, so they and O are held in units of 2^qe, the
+        // largest (scaled) step seen, 1 at least: weights, up to 2^15, and their products with steps stay in f16's range.
         // A step of 64 or more is infinite here: rows that see one are computed again
         int qe = 0;
         wf4 t[2];
@@ -868,7 +879,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
             }
             wf4 one[1] = {wf4{f, 0.f, 0.f, 0.f}};               // O's factor
             const float ms = fw_raise<1>(s, m, l, one);
-            const float qf = QUANT ? __builtin_amdgcn_ldexpf(1.f, 7 - qe) : 1.f;
+            const float qf = QUANT ? __builtin_amdgcn_ldexpf(1.f, -qe) : 1.f;
             const wf4 sv = dh ? s[1] : s[0];
             wf4 e;
 #pragma unroll
@@ -979,7 +990,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
     }
     fw_barrier();
     if constexpr (QUANT) {
-        const float f = __builtin_amdgcn_ldexpf(1.f, endq - 7 - FQ_STEP);
+        const float f = __builtin_amdgcn_ldexpf(1.f, endq - FQ_STEP);
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= f;
     }
