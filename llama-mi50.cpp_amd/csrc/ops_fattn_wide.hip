@@ -676,10 +676,15 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
         const uint32_t x = KV == GGML_TYPE_Q8_0 ? u.x ^ 0x80808080u : u.x & k.mask, y = KV == GGML_TYPE_Q8_0 ? u.y ^ 0x80808080u : u.y & k.mask;
         return make_uint4(pair(x, 0, k), pair(x, 1, k), pair(y, 0, k), pair(y, 1, k));
     };
+    // a step past f16's range (64, or no number) becomes a NaN: as an infinity in a block that only K has, it would take a
+    // visible key's score to -inf as soon as to +inf, and nothing would tell
+    auto scaled = [](_Float16 d) __attribute__((always_inline)) {
+        return __builtin_fabsf((float) d) < 65536.f / (1 << FQ_STEP) ? d * (_Float16) (1 << FQ_STEP) : (_Float16) __builtin_nanf("");
+    };
     auto store = [&](const Regs & q, int slot, int half) __attribute__((always_inline)) {
         char * const buf = ring + slot * FQ_BUF;
         _Float16 * const steps = (_Float16 *) (buf + 9 * FW_PIECE);
-        steps[(x8 + 8 * half) * FW_KT + row] = q.d[half] * (_Float16) (1 << FQ_STEP);
+        steps[(x8 + 8 * half) * FW_KT + row] = scaled(q.d[half]);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             *(uint4 *) (buf + at[c] + 4 * half * FW_PIECE) = chunk(q.a[half][c & (NL - 1)], c == 0 ? n0 : c == 1 ? n1 : c == 2 ? n2 : n3);
@@ -688,7 +693,7 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
             if (lane == 0) dtop[slot][wave] = top;
             return;
         }
-        steps[pblk * FW_KT + row] = q.d[2] * (_Float16) (1 << FQ_STEP);
+        steps[pblk * FW_KT + row] = scaled(q.d[2]);
         *(uint4 *) (buf + 8 * FW_PIECE + 128 * row + 16 * (x8 ^ sw)) = chunk(q.w, pnib);
     };
 
@@ -809,7 +814,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
         float m = -INFINITY, l = 0.f;
         // the weights take V's steps before they are split, so they and O are held in units of 2^qe, the
         // largest (scaled) step seen, 1 at least: weights, up to 2^15, and their products with steps stay in f16's range.
-        // A step of 64 or more is infinite here: rows that see one are computed again
+        // A step of 64 or more is a NaN here: rows that see one are computed again
         int qe = 0;
         wf4 t[2];
         auto scores = [&](const char * buf) __attribute__((always_inline)) {
