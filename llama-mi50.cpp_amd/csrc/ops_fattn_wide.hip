@@ -34,6 +34,7 @@ typedef _Float16 wh8 __attribute__((ext_vector_type(8)));
 typedef _Float16 wh4 __attribute__((ext_vector_type(4)));
 typedef _Float16 wh2 __attribute__((ext_vector_type(2)));
 typedef float wf4 __attribute__((ext_vector_type(4)));
+typedef uint16_t wu4 __attribute__((ext_vector_type(4)));
 typedef __fp16 w16x4 __attribute__((vector_size(8)));
 typedef __attribute__((address_space(3))) w16x4 * lds_w4;
 typedef __attribute__((address_space(3))) void * lds_dma;
@@ -122,6 +123,14 @@ template <bool SUM> __device__ __forceinline__ float fw_row4(float x) {
     x = SUM ? __uint_as_float(a.x) + __uint_as_float(a.y) : fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
     a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return SUM ? __uint_as_float(a.x) + __uint_as_float(a.y) : fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
+}
+
+__device__ __forceinline__ uint32_t fw_row4_max(uint32_t x) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    u2 a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(a.x, a.y);
+    a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max(a.x, a.y);
 }
 
 // element i of a cache row, for the plain loop below
@@ -634,12 +643,12 @@ constexpr int FQ_STEP = 10;                                     // ... times 2^1
 
 // the last kind, quantised: blocks through registers, two tiles ahead of the store
 template <int KV, int ROWS>
-__device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, char * ring, float (&dtop)[3][4]) {
+__device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, char * ring, uint16_t (&vtop)[3][FW_KT]) {
     // eight threads a row take two whole 32-blocks each, x and x + 8, and eight values of the last two blocks. A block
     // goes to LDS in four chunks of 8 values, thread x starting with the rot-th: the same chunk of all eight blocks
     // would lie in the same banks (1160 of a tile's 2700 LDS cycles were conflicts)
     constexpr int QB = qsize_of<KV>(), NL = KV == GGML_TYPE_Q8_0 ? 4 : 2;      // 8-byte loads of a block
-    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x & 255;
     const int row = tid >> 3, x8 = tid & 7, sw = fw_swz(row), pblk = 16 + (x8 >> 2), pval = 8 * (x8 & 3), rot = x8 >> 1;
     int at[4], from[NL];                                        // places of the chunks, sources of the loads
 #pragma unroll
@@ -655,6 +664,7 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
     };
     const Nib n0 = nibble(rot & 2), n1 = nibble((rot + 1) & 2), n2 = nibble(!(rot & 2)), n3 = nibble(!((rot + 1) & 2)), pnib = nibble(pval & 16);
     struct Regs { uint2 a[2][NL], w; _Float16 d[3]; } set[2];
+    const uint32_t m0 = p.vpiece && x8 < 2 ? 0 : 0x7FFF, m2 = p.vpiece ? 0x7FFF : 0;
     auto load = [&](int tile, Regs & q) __attribute__((always_inline)) {
         const int key0 = (tile & FW_TILE) * FW_KT;
         const char * kb = j.kb + (size_t) key0 * p.k1;          // (uniform; a lane's offset has 32 bits)
@@ -689,8 +699,13 @@ __device__ __forceinline__ void fw_produce(const FwArgs & p, const FwJob & j, ch
         for (int c = 0; c < 4; ++c)
             *(uint4 *) (buf + at[c] + 4 * half * FW_PIECE) = chunk(q.a[half][c & (NL - 1)], c == 0 ? n0 : c == 1 ? n1 : c == 2 ? n2 : n3);
         if (half == 0) {
-            const float top = wave_max<64>(fmaxf(fmaxf(fabsf((float) q.d[0]), fabsf((float) q.d[1])), fabsf((float) q.d[2])));
-            if (lane == 0) dtop[slot][wave] = top;
+            // the largest step of each key's values: all blocks but the last two or, vpiece, but the first two
+            const uint32_t b0 = __builtin_bit_cast(uint16_t, q.d[0]), b1 = __builtin_bit_cast(uint16_t, q.d[1]), b2 = __builtin_bit_cast(uint16_t, q.d[2]);
+            int top = max(max(b0 & m0, b1 & 0x7FFF), b2 & m2);
+            top = max(top, dpp_i<0xB1>(0, top));
+            top = max(top, dpp_i<0x4E>(0, top));
+            top = max(top, dpp_i<0x141>(0, top));
+            if (x8 == 0) vtop[slot][row] = (uint16_t) top;
             return;
         }
         steps[pblk * FW_KT + row] = scaled(q.d[2]);
@@ -785,15 +800,15 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
     __shared__ __align__(16) wf4 exch[4][2][64];                // halves of scores
     __shared__ __align__(16) wf4 wgt[2][2][64];                 // weights: row group, 16 keys, the scores' lane
     __shared__ float scl[2][16];                                // a row's O takes this factor before them
-    __shared__ __align__(16) float dtop[3][4];                  // the tiles' largest steps, wave by wave
+    __shared__ __align__(16) uint16_t vtop[3][FW_KT];           // the largest step of each key's values, as f16's bits
     __shared__ float endm[2][64], endl[2][2][64];
-    __shared__ int endq;
+    __shared__ int endq[2][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n16 = lane & 15, g4 = lane >> 4, rg = wave >> 1 & 1, dh = wave & 1;
     const FwJob j = fw_job<ROWS, false>(p);
     if (wave >= 8) {
         __builtin_amdgcn_s_setprio(2);                          // (the longest of the three; without it 49 us instead of 47)
-        if constexpr (QUANT) fw_produce<KV, ROWS>(p, j, ring, dtop);
+        if constexpr (QUANT) fw_produce<KV, ROWS>(p, j, ring, vtop);
         else fw_fetch<ROWS>(p, j, ring);
         return;
     }
@@ -812,8 +827,9 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
         const int kx0 = 128 * n16 + 16 * (g4 ^ fw_swz(n16)), kx1 = 128 * n16 + 16 * ((4 + g4) ^ fw_swz(n16));
         const int ka0 = dh ? kx1 + 4 * FW_PIECE : kx0, ka1 = dh ? kx0 + 5 * FW_PIECE : kx1;
         float m = -INFINITY, l = 0.f;
-        // the weights take V's steps before they are split, so they and O are held in units of 2^qe, the
-        // largest (scaled) step seen, 1 at least: weights, up to 2^15, and their products with steps stay in f16's range.
+        // the weights take V's steps before they are split, so they and O are held in units of 2^qe, the largest (scaled)
+        // step in the values of a key that the row sees, 1 at least: weights, up to 2^15, and their products with steps stay
+        // in f16's range. (What other keys hold, and the channels that only K has, would cost the weights their last bits.)
         // A step of 64 or more is a NaN here: rows that see one are computed again
         int qe = 0;
         wf4 t[2];
@@ -873,14 +889,14 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
             if (tile >> 30) fw_mask(p, j, r, tile & FW_TILE, s);
             float f = 1.f;
             if constexpr (QUANT) {
-                float top = 0.f;
+                const wu4 d[2] = {*(const wu4 *) &vtop[slot][4 * g4], *(const wu4 *) &vtop[slot][16 + 4 * g4]};
+                uint32_t top = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, dtop[slot][i]);
-                const int x = top < INFINITY ? __builtin_amdgcn_frexp_expf(top) + FQ_STEP : 0;
-                if (x > qe) {                                   // the same in every wave; on the first tiles only
-                    f = __builtin_amdgcn_ldexpf(1.f, qe - x);
-                    qe = x;
-                }
+                for (int i = 0; i < 8; ++i) top = max(top, s[i >> 2][i & 3] == -INFINITY ? 0u : (uint32_t) d[i >> 2][i & 3]);
+                // an exponent as frexp has it; below f16's normal range (0) it raises nothing, and rows that see a NaN start again
+                const int x = max((int) (fw_row4_max(top) >> 10) - 14 + FQ_STEP, qe);
+                f = __builtin_amdgcn_ldexpf(1.f, qe - x);       // the same in both waves of the row; 1 but on its first tiles
+                qe = x;
             }
             wf4 one[1] = {wf4{f, 0.f, 0.f, 0.f}};               // O's factor
             const float ms = fw_raise<1>(s, m, l, one);
@@ -906,7 +922,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
         }
         endl[rg][dh][lane] = l;
         if (dh == 0) endm[rg][lane] = m;
-        if (wave == 0 && lane == 0) endq = qe;
+        if (dh == 0 && g4 == 0) endq[rg][n16] = qe;
         fw_barrier();
         return;
     }
@@ -995,7 +1011,7 @@ __global__ __launch_bounds__(768, 3) void k_fattn_latent32(FwArgs p) {
     }
     fw_barrier();
     if constexpr (QUANT) {
-        const float f = __builtin_amdgcn_ldexpf(1.f, endq - FQ_STEP);
+        const float f = __builtin_amdgcn_ldexpf(1.f, endq[rg][n16] - FQ_STEP);
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= f;
     }
