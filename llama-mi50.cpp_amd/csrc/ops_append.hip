@@ -427,6 +427,8 @@ int fuse_append_rows(OpCtx & c, ggml_cgraph * g, int i, const UseCount & use_map
         if (through_views(sk->src[0]) != cat || !single(cat, sk->src[0])) return 0;
     } else return 0;
 
+    // a member in place (a view of its input) leaves its result there, which the one launch would not
+    for (const ggml_tensor * t : {rope, norm, mul, cat}) if (t && t->view_src) return 0;
     AppendP p{};
     const ggml_tensor * x = rope->src[0];
     const int64_t ntok = x->ne[2];

@@ -1,5 +1,5 @@
 """Cache rows appended with the rotation on the way, from graphs that look like the ones fused and are not quite: factors of
-another shape, members over memory that died."""
+another shape, members over memory that died, members in place."""
 import numpy as np
 import pytest
 
@@ -69,3 +69,19 @@ def test_members_over_memory_that_died(ctx, backend, member, mode):
     bound = np.concatenate([tol, (10 + 19) * EPS32 * mag], 1)
     assert np.all(np.abs(got[3:3 + n] - want) <= bound + EPS16 * (np.abs(want) + bound) + 2.0 ** -25) and not got[:3].any() and not got[3 + n:].any()
     assert np.all(np.abs(twice.numpy().reshape(n, 512) - 2 * kept) <= 64 * EPS32 * np.abs(kept))
+
+
+def test_rotation_in_place(ctx, backend):
+    """keys turned in place (ggml_rope_ext_inplace: a view of its input) and appended: the keys themselves turn too"""
+    rng = np.random.default_rng(0)
+    n, heads, dim = 7, 2, 64
+    k, pos, kc, ix = ctx.new_tensor("f32", dim, heads, n), ctx.new_tensor("i32", 4 * n), ctx.new_tensor("f16", dim * heads, 16), ctx.new_tensor("i64", n)
+    turned = rope_node(ctx, k, pos, MROPE, dim)
+    turned.raw.view_src = k.ptr
+    out = ctx.set_rows(kc, ctx.reshape(turned, dim * heads, n), ix)
+    ks, p = rng.standard_normal((n, heads, dim)).astype(np.float32), positions(n, rng)
+    got = run(ctx, backend, [out], [(k, ks), (pos, p), (ix, np.arange(n)), (kc, np.zeros((16, dim * heads), np.float16))])[0].reshape(16, -1)
+    want, mag = rope_want(ks, p, MROPE, dim)
+    bound = 10 * EPS32 * mag
+    assert np.all(np.abs(k.numpy().reshape(n, heads, dim) - want) <= bound)
+    assert np.all(np.abs(got[:n].reshape(n, heads, dim) - want) <= bound + EPS16 * (np.abs(want) + bound) + 2.0 ** -25)
