@@ -89,6 +89,8 @@ __global__ __launch_bounds__(256) void k_rope_axes(const char * __restrict__ x, 
     }
 }
 
+constexpr int64_t MX_MAX_TOKENS = UINT32_MAX / 256;            // a launch counts its threads in 32 bits: workgroups of 256, one a token
+
 static bool rope_pos_ok(const ggml_tensor * dst) {
     const ggml_tensor * x = dst->src[0], * pos = dst->src[1], * ff = dst->src[2];
     const int mode = mx_op_param<int32_t>(dst, 2), n_dims = mx_op_param<int32_t>(dst, 1);
@@ -119,7 +121,7 @@ bool rope_axes_supported(const ggml_tensor * dst) {
         }
         default: return false;
     }
-    if (rope_pairs(mode, n_dims) > MX_ROPE_MAXP || x->ne[0] * x->ne[1] > INT32_MAX / 2 || x->ne[2] * x->ne[3] > INT32_MAX) return false;
+    if (rope_pairs(mode, n_dims) > MX_ROPE_MAXP || x->ne[0] * x->ne[1] > INT32_MAX / 2 || x->ne[2] * x->ne[3] > MX_MAX_TOKENS) return false;
     return rope_pos_ok(dst);
 }
 
@@ -475,7 +477,7 @@ int fuse_append_rows(OpCtx & c, ggml_cgraph * g, int i, const UseCount & use_map
         last = at[2];
     } else { sv = nullptr; p.v.width = 0; }
     if (!sv && !fused_io_ok({sk, keep_mul ? mul : nullptr}, {x, rope->src[1], rope->src[2], sk->src[1], nx, w})) return 0;
-    if (p.k.width > APPEND_MAX_ROW || ntok > INT32_MAX) return 0;
+    if (p.k.width > APPEND_MAX_ROW || ntok > MX_MAX_TOKENS) return 0;
     kv_new_row_flush(c);                                        // (its cache may be the one written here)
     for (int j = i; j <= last; ++j) {
         deferred_guard_node_ext(c, g->nodes[j]);
