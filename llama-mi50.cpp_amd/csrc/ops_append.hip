@@ -76,8 +76,14 @@ __global__ __launch_bounds__(256) void k_rope_axes(const char * __restrict__ x, 
             T & b = !ADJ || V == 1 ? ahi.v[j] : (2 * j < V ? alo.v[(2 * j + 1) % V] : ahi.v[(2 * j + 1) % V]);
             const float2 t = tab[i + j];
             const float x0 = rd<T>(a), x1 = rd<T>(b);
-            a = wr<T>(x0 * t.x - x1 * t.y);
-            b = wr<T>(x0 * t.y + x1 * t.x);
+            if constexpr (std::is_same<T, float>::value) {      // (rows in f32 are the ones that an append turns as well)
+                const float2 v = rope_turn<true>(x0, x1, t);
+                a = v.x;
+                b = v.y;
+            } else {
+                a = wr<T>(x0 * t.x - x1 * t.y);
+                b = wr<T>(x0 * t.y + x1 * t.x);
+            }
         }
         stv<T, V>(ry + (ADJ ? 2 * i : i), alo);
         stv<T, V>(ry + (ADJ ? 2 * i + V : i + np), ahi);
@@ -228,7 +234,7 @@ struct RowDst {
 };
 struct AppendP {
     const char * nx; size_t n_tok; const float * nw; char * nout; size_t nout_tok; int n_norm, norm_at; float eps;   // n_norm = 0: none
-    const char * rx; size_t r_head, r_tok; const int32_t * pos; const float * ff; int heads, dim, rot_at, np, adj; int64_t ntok;
+    const char * rx; size_t r_head, r_tok; const int32_t * pos; const float * ff; int heads, dim, rot_at, np, adj, by_token; int64_t ntok;
     RopeP rope;
     const char * vx; size_t v_tok; int v4;                      // v4: rows of whole 16 bytes, aligned
     RowDst k, v;
@@ -343,10 +349,10 @@ __global__ __launch_bounds__(256) void k_append_rows(AppendP p) {
     __syncthreads();                                            // the table
     auto turn = [&](int u, float x0, float x1) {
         const int h = u / p.np, i = u % p.np;
-        const float2 cs = tab[i];
+        const float2 v = p.by_token ? rope_turn<true>(x0, x1, tab[i]) : rope_turn<false>(x0, x1, tab[i]);
         float * r = row + p.rot_at + h * p.dim;
-        r[p.adj ? 2 * i : i] = x0 * cs.x - x1 * cs.y;
-        r[p.adj ? 2 * i + 1 : i + p.np] = x0 * cs.y + x1 * cs.x;
+        r[p.adj ? 2 * i : i] = v.x;
+        r[p.adj ? 2 * i + 1 : i + p.np] = v.y;
     };
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) if (tid + a * nt < pairs) turn(tid + a * nt, r0[a], r1[a]);
@@ -441,7 +447,7 @@ int fuse_append_rows(OpCtx & c, ggml_cgraph * g, int i, const UseCount & use_map
     if (p.np < 1 || p.np > MX_ROPE_MAXP || 2 * p.np > x->ne[0]) return 0;
     p.rx = (const char *) x->data; p.r_head = x->nb[1]; p.r_tok = x->nb[2];
     p.pos = (const int32_t *) rope->src[1]->data; p.ff = rope->src[2] ? (const float *) rope->src[2]->data : nullptr;
-    p.dim = (int) x->ne[0]; p.adj = p.rope.mode == GGML_ROPE_TYPE_NORMAL; p.ntok = ntok;
+    p.dim = (int) x->ne[0]; p.adj = p.rope.mode == GGML_ROPE_TYPE_NORMAL; p.by_token = rope_has_axes(p.rope.mode) || rope_by_token(rope); p.ntok = ntok;
     if (x->ne[0] * x->ne[1] > APPEND_MAX_ROW) return 0;
     p.heads = (int) x->ne[1];
     const int turned = p.heads * p.dim;

@@ -827,6 +827,11 @@ __global__ __launch_bounds__(256) void k_rope2(const char * __restrict__ x, cons
     }
 }
 
+bool rope_by_token(const ggml_tensor * dst) {
+    const ggml_tensor * x = dst->src[0];
+    return x->ne[2] * x->ne[3] > 1 && x->ne[1] > 1 && mx_op_param<int32_t>(dst, 1) / 2 <= MX_ROPE2_MAXP && x->ne[0] % 2 == 0 && !g_rope1;
+}
+
 void op_rope(OpCtx & c, ggml_tensor * dst) {
     const ggml_tensor * x = dst->src[0];
     const ggml_tensor * pos = dst->src[1];
@@ -836,7 +841,7 @@ void op_rope(OpCtx & c, ggml_tensor * dst) {
     const int bs = 64;
     const float * pff = ff ? (const float *) ff->data : nullptr;
     const bool neox = (p.mode & GGML_ROPE_TYPE_NEOX) != 0;
-    if (x->ne[2] * x->ne[3] > 1 && x->ne[1] > 1 && p.n_dims / 2 <= MX_ROPE2_MAXP && x->ne[0] % 2 == 0 && !g_rope1) {
+    if (rope_by_token(dst)) {
         const unsigned g = (unsigned) (x->ne[2] * x->ne[3]);
 #define R2(T, NX) k_rope2<T, NX><<<g, 256, 0, c.st>>>((const char *) x->data, (const int32_t *) pos->data, pff, (char *) dst->data, geo(x), geo(dst), p)
         if (x->type == GGML_TYPE_F32) { if (neox) R2(float, true); else R2(float, false); }

@@ -47,7 +47,17 @@ static inline RopeP rope_params(const ggml_tensor * dst) {
     return p;
 }
 
+// ROPE of one axis by a workgroup a token rather than a row (op_rope, ops_misc.hip)
+bool rope_by_token(const ggml_tensor * dst);
+
 #if defined(__HIPCC__)
+// The pair (x0, x1) turned by t = (cos, sin): (x0 cos - x1 sin, x0 sin + x1 cos). A sum of two products may round either of
+// them first, as a compiler likes, so what has to give the same bits in several kernels is written out: TOKEN as in the
+// kernels that take a token at a time, else as in the one that takes a row
+template <bool TOKEN> __device__ __forceinline__ float2 rope_turn(float x0, float x1, float2 t) {
+    return make_float2(__builtin_fmaf(x0, t.x, -(x1 * t.y)), TOKEN ? __builtin_fmaf(x0, t.y, x1 * t.x) : __builtin_fmaf(x1, t.x, x0 * t.y));
+}
+
 __device__ __forceinline__ void rope_cs(float theta_extrap, const RopeP & p, int i0, float * c, float * s) {
     const float theta_interp = p.freq_scale * theta_extrap;
     float theta = theta_interp;
