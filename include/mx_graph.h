@@ -96,7 +96,8 @@ size_t mxg_nbytes(const struct ggml_tensor * t);
 
 enum ggml_status mxg_compute(ggml_backend_t backend, struct ggml_cgraph * g);
 /* as mxg_compute, without waiting (ggml_backend_graph_compute_async): the work is queued on the backend's
- * stream, in order with earlier graphs; mxg_synchronize waits for it */
+ * stream, in order with earlier graphs; mxg_synchronize waits for it. Inputs are set again, and results read, only behind
+ * that wait */
 enum ggml_status mxg_compute_async(ggml_backend_t backend, struct ggml_cgraph * g);
 void mxg_synchronize(ggml_backend_t backend);
 void mxg_backend_free(ggml_backend_t backend);

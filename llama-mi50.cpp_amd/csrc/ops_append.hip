@@ -162,7 +162,8 @@ void op_rope_axes(OpCtx & c, ggml_tensor * dst) {
 
 // ---------------------------------------------------------------------------
 // CONCAT along one dimension: every element (or 16 bytes of a row) of the result is read from the
-// operand that owns its index
+// operand that owns its index. Two halves of 8.4 MB along dimension 2 7.0 us (4.8 TB/s), 2011 rows of 512 and 64 in f32 3.9; element
+// by element the index arithmetic bounds it: rows of 512 and 63 7.0 us
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void k_concat(const char * __restrict__ a, const char * __restrict__ b, char * __restrict__ y, G4 ga, G4 gb, G4 gy,
@@ -224,8 +225,9 @@ void op_concat(OpCtx & c, ggml_tensor * dst) {
 // (keys); a second, unturned row (values) may go to a cache of its own. The row is assembled in LDS in
 // 32 bits and rounded once into the cache's type. Against the separate launches (RMS_NORM + MUL, ROPE,
 // CONCAT, SET_ROWS) it saves their round trips through memory, and at a token or two the launches. The chain fetch, sum,
-// rotate, store of a row bounds it: 8 latent rows 5.1 us, 2011 6.5 us (7 MB), 512 rows of keys and of values 5.4 us; 1800 rows of
-// 16 heads of keys and of values in f32, 59 MB, 14.6 us.
+// rotate, store of a row bounds it: 8 latent rows 4.7 us, 2011 6.3 us (7 MB), 512 rows of keys and of values 5.4 us; 1800 rows of
+// 16 heads of keys and of values in f32, 59 MB, 14.6 us. With one axis a table's recurrence adds 0.6 us. Rows in 8 and 4 bits are
+// rounded by a thread a block (18 of a latent row's 192): 0.7 and 0.5 us more than f16.
 // ---------------------------------------------------------------------------
 struct RowDst {
     char * base; size_t nb1; int64_t ne1; int type;             // a cache

@@ -254,7 +254,8 @@ class Context:
             raise MemoryError("mxg_alloc failed")
 
     def compute_async(self, backend, graph):
-        """compute() without the wait: queued on the backend's stream, in order with its other graphs."""
+        """compute() without the wait: queued on the backend's stream, in order with its other graphs. Backend.synchronize
+        waits; inputs are set again, and results read, only behind it."""
         st = self.lib.mxg_compute_async(backend.ptr, graph)
         if st != 0:
             raise RuntimeError(f"graph_compute returned status {st}")
